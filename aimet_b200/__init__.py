@@ -9,6 +9,8 @@
 * :mod:`aimet_b200.float_quantizer` -- ``FloatQuantizeDequantize`` (fp16 / bf16 / fp8 / fp4 fake-cast), MXFP4, NVFP4.
 * :mod:`aimet_b200.encoding_analyzer` -- MinMax / Percentile / SQNR / TF-enhanced analyzers.
 * :mod:`aimet_b200.seq_mse` -- SeqMSE candidate search for Linear layers.
+* :mod:`aimet_b200.int4` -- products with packed 4-bit weights (what the 4-bit quantizers calibrate).
+* :mod:`aimet_b200.kv_cache` -- a paged 8-bit key / value cache and attention over it.
 * :mod:`aimet_b200.distributed` -- sharded calibration and output-channel sharding helpers.
 
 Everything runs through ``libaimet_b200.so`` (``include/aimet_b200.h``); importing the package
@@ -18,12 +20,12 @@ fails if that library has not been built (``python -m aimet_b200.build``).
 import importlib
 
 __all__ = [
-    "backend", "functional", "quantizer", "float_quantizer", "encoding_analyzer", "seq_mse", "distributed", "nn",
+    "backend", "functional", "quantizer", "float_quantizer", "encoding_analyzer", "seq_mse", "int4", "kv_cache", "distributed", "nn",
     "quantize", "dequantize", "quantize_dequantize", "register_backend",
 ]
 
-_SUBMODULES = ("_lib", "backend", "functional", "pgs", "quantizer", "float_quantizer", "encoding_analyzer", "seq_mse", "distributed", "nn",
-               "build")
+_SUBMODULES = ("_lib", "backend", "functional", "pgs", "quantizer", "float_quantizer", "encoding_analyzer", "seq_mse", "int4", "kv_cache", "distributed",
+               "nn", "build")
 _FUNCTIONS = ("quantize", "dequantize", "quantize_dequantize")
 
 

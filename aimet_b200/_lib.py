@@ -43,6 +43,39 @@ class Layout(ctypes.Structure):
     ]
 
 
+class Int4Weight(ctypes.Structure):
+    """Mirror of ``ab_int4_weight``."""
+
+    _fields_ = [
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("block", ctypes.c_int32),
+        ("scale_kind", ctypes.c_int32),
+        ("zero", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+        ("zeros", ctypes.c_void_p),
+        ("row_scale", ctypes.c_void_p),
+    ]
+
+
+class KVCache(ctypes.Structure):
+    """Mirror of ``ab_kv_cache``."""
+
+    _fields_ = [
+        ("key", ctypes.c_void_p),
+        ("value", ctypes.c_void_p),
+        ("key_scale", ctypes.c_void_p),
+        ("value_scale", ctypes.c_void_p),
+        ("num_pages", ctypes.c_int64),
+        ("num_heads", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 def make_layout(size: Sequence[int], block: Sequence[int]) -> Layout:
     if len(size) != len(block):
         raise ValueError("size and block must have the same length")
@@ -72,6 +105,8 @@ _i32 = ctypes.c_int
 _i64 = ctypes.c_int64
 _f64 = ctypes.c_double
 _lay = ctypes.POINTER(Layout)
+_w4 = ctypes.POINTER(Int4Weight)
+_kvc = ctypes.POINTER(KVCache)
 
 # name -> (restype, argtypes); kept in one table so a test can check it against the header
 SIGNATURES = {
@@ -149,6 +184,16 @@ SIGNATURES = {
     "aimet_b200_seqmse_linear_loss": (
         _i32,
         [_vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp],
+    ),
+    "aimet_b200_int4_codes_bytes": (_i64, [_i64, _i64]),
+    "aimet_b200_int4_pack": (_i32, [_vp, _i64, _i64, _i32, _vp, _vp]),
+    "aimet_b200_int4_linear": (_i32, [_w4, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "aimet_b200_kv_append": (_i32, [_kvc, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp]),
+    "aimet_b200_kv_gather": (_i32, [_kvc, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
+    "aimet_b200_kv_attention_scratch_bytes": (_i64, [_kvc, _i64, _i64, _i64, _i64, _i32]),
+    "aimet_b200_kv_attention": (
+        _i32,
+        [_kvc, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i64, _f64, _i32, _vp, _i64, _vp],
     ),
 }
 

@@ -1,0 +1,213 @@
+"""Products with 4-bit weights: inference on what the 4-bit weight quantizers calibrate.
+
+:class:`PackedInt4Weight` holds the codes of a ``[out_features, in_features]`` weight in four bits with
+their scales (per channel, blockwise along the input channels, or the blockwise grid of
+``GroupedBlockQuantizeDequantize`` whose scales are small integers times a per-channel scale), and
+:func:`linear_int4` multiplies with it without ever writing the weight out in 16 bits.  The grids and
+their names follow aimet_torch (quantization/affine/quantizer.py:1072-1440, affine/encoding.py:560-620);
+the reference itself only simulates them.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from . import _lib, backend
+from ._lib import check, lib
+
+__all__ = ["PackedInt4Weight", "linear_int4"]
+
+_TILE_N, _TILE_K = 16, 64
+_MAX_ZERO = 112  # 16-bit floats subtract zero points up to here exactly
+
+
+def _storage_block(block: int, in_features: int) -> int:
+    """Input channels per scale as the kernels store them: 16, 32 or a multiple of 64 that divides
+    ``block``; a scale for the whole row counts as the next multiple of 64."""
+    if block == in_features:
+        return -(-in_features // _TILE_K) * _TILE_K
+    for b in (64, 32, 16):
+        if block % b == 0:
+            return block if b == 64 else b
+    raise NotImplementedError(f"blocks of {block} input channels: a multiple of 16, or the whole row, is supported")
+
+
+def _tiled(param: torch.Tensor, block: int, storage: int, in_features: int) -> torch.Tensor:
+    """[out, blocks] -> the kernels' order [ceil(out / 16)][entries][16][sub] (zeros behind the matrix)."""
+    n = param.shape[0]
+    sub = max(1, _TILE_K // storage)
+    tiles = -(-in_features // _TILE_K)
+    entries = -(-tiles // max(1, storage // _TILE_K))
+    if block != in_features and storage != block:
+        param = param.repeat_interleave(block // storage, 1)
+    out = param.new_zeros(-(-n // _TILE_N) * _TILE_N, entries * sub)
+    out[:n, : param.shape[1]] = param
+    return out.view(-1, _TILE_N, entries, sub).permute(0, 2, 1, 3).contiguous()
+
+
+class PackedInt4Weight:
+    """4-bit codes of a linear layer's weight with their scales, laid out for the CUDA kernels.
+
+    Made by :meth:`from_codes`, :meth:`from_encoding` or :meth:`from_quantizer`; its contents are fixed.
+    ``w[n, k] = (code[n, k] + offset[n, b]) * scale[n, b]`` with ``b`` the block of column ``k``.
+    """
+
+    def __init__(self, out_features, in_features, block_size, qmin, codes, scales, zeros, row_scale, zero):
+        self.out_features, self.in_features = out_features, in_features
+        self.block_size, self.qmin = block_size, qmin
+        self._buffers = (codes, scales, zeros, row_scale)  # what the descriptor below points at
+        storage = _storage_block(block_size, in_features)
+        self._desc = _lib.Int4Weight(out_features, in_features, storage, int(row_scale is not None), zero, 0,
+                                     codes.data_ptr(), scales.data_ptr(), _lib.ptr(zeros), _lib.ptr(row_scale))
+        self.device = codes.device
+
+    @property
+    def nbytes(self) -> int:
+        """Bytes on the device."""
+        return sum(t.numel() * t.element_size() for t in self._buffers if t is not None)
+
+    def __repr__(self):
+        return (f"PackedInt4Weight({self.out_features}x{self.in_features}, block_size={self.block_size}, "
+                f"device={self.device})")
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scale: torch.Tensor, offset: Optional[torch.Tensor] = None, *,
+                   qmin: int = -8, int_scale: Optional[torch.Tensor] = None) -> "PackedInt4Weight":
+        """From codes ``[out_features, in_features]`` (whole numbers in ``[qmin, qmin + 15]``, any dtype).
+
+        ``scale``: ``[out_features, blocks]`` (``blocks == 1``: per channel); ``offset``: the same shape,
+        whole numbers, or None for zeros.  With ``int_scale`` (``[out_features, blocks]``, whole numbers in
+        ``[0, 255]``) the scale of a block is ``int_scale * scale`` and ``scale`` is ``[out_features, 1]``.
+        Checks the values, which waits for the device: pack a weight once, not per forward.
+        """
+        if codes.dim() != 2 or codes.numel() == 0:
+            raise RuntimeError(f"codes must be a non-empty matrix, got shape {tuple(codes.shape)}")
+        if not codes.is_cuda:
+            raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
+        n, k = codes.shape
+        qmin = int(qmin)
+        if not -128 <= qmin <= 112:
+            raise RuntimeError(f"codes of [{qmin}, {qmin + 15}] do not fit signed bytes")
+        per_block = scale if int_scale is None else int_scale
+        if per_block.dim() != 2 or per_block.shape[0] != n or per_block.shape[1] < 1 or k % per_block.shape[1]:
+            raise RuntimeError(f"scales of shape {tuple(per_block.shape)} do not divide a weight of shape {(n, k)}")
+        if int_scale is not None and tuple(scale.shape) != (n, 1):
+            raise RuntimeError(f"with int_scale, scale must have shape {(n, 1)}, got {tuple(scale.shape)}")
+        if offset is not None and tuple(offset.shape) != tuple(per_block.shape):
+            raise RuntimeError(f"offset must have shape {tuple(per_block.shape)}, got {tuple(offset.shape)}")
+        for t in (scale, offset, int_scale):
+            if t is not None and t.device != codes.device:
+                raise RuntimeError(f"expected all tensors on {codes.device}, got {t.device}")
+        with torch.no_grad():
+            block = k // per_block.shape[1]
+            storage = _storage_block(block, k)
+            whole = codes.to(torch.int32)
+            if bool(((whole != codes) | (whole < qmin) | (whole > qmin + 15)).any()):
+                raise RuntimeError(f"codes must be whole numbers in [{qmin}, {qmin + 15}]")
+            row_scale = None
+            if int_scale is None:
+                scales = _tiled(scale.detach().to(torch.float32), block, storage, k)
+            else:
+                if bool(((int_scale != int_scale.to(torch.uint8)) | (int_scale < 0) | (int_scale > 255)).any()):
+                    raise RuntimeError("int_scale must hold whole numbers in [0, 255]")
+                scales = _tiled(int_scale.to(torch.uint8), block, storage, k)
+                row_scale = scale.detach().to(torch.float32).reshape(-1).contiguous().clone()
+            zeros, zero = None, -qmin
+            if offset is not None:
+                z = -(offset.detach().double() + qmin)
+                if bool(((z != z.round()) | (z.abs() > _MAX_ZERO)).any()):
+                    raise NotImplementedError(f"offsets must be whole numbers with |offset + qmin| <= {_MAX_ZERO}")
+                if bool((z == z[0, 0]).all()):
+                    zero = int(z[0, 0].item())
+                else:
+                    zeros = _tiled(z.to(torch.int8), block, storage, k)
+            elif abs(zero) > _MAX_ZERO:
+                raise NotImplementedError(f"qmin={qmin} without an offset: |qmin| <= {_MAX_ZERO} is supported")
+            codes8 = whole.to(torch.int8).contiguous()
+            packed = torch.empty(lib.aimet_b200_int4_codes_bytes(n, k), dtype=torch.uint8, device=codes.device)
+            with _lib.on_device(codes.device):
+                check(lib.aimet_b200_int4_pack(codes8.data_ptr(), n, k, qmin, packed.data_ptr(), _lib.stream_ptr(codes.device)))
+        return cls(n, k, block, qmin, packed, scales, zeros, row_scale, zero)
+
+    @classmethod
+    def from_encoding(cls, weight: torch.Tensor, encoding) -> "PackedInt4Weight":
+        """Quantize ``weight`` ``[out_features, in_features]`` with a 4-bit ``AffineEncoding`` (per tensor, per
+        output channel, or blockwise along the input channels) and pack the codes."""
+        if weight.dim() != 2:
+            raise NotImplementedError(f"weights of linear layers are packed, got shape {tuple(weight.shape)}")
+        if encoding.qmax - encoding.qmin > 15:
+            raise NotImplementedError(f"a grid of [{encoding.qmin}, {encoding.qmax}] does not fit 4 bits")
+        if encoding.zero_point_shift:
+            raise NotImplementedError("a grid with a zero-point shift cannot be packed")
+        n, k = weight.shape
+        scale, offset = encoding.scale, encoding.offset
+        with torch.no_grad():
+            codes = backend.quantize(weight.detach(), scale, offset, encoding.qmin, encoding.qmax, encoding.block_size)
+            if scale.dim() > 2:
+                raise NotImplementedError(f"scales of shape {tuple(scale.shape)} for a linear layer's weight")
+
+            def per_channel(p):  # [out or 1, blocks] -> [out, blocks]
+                p = p.detach().to(torch.float32).reshape((1,) * (2 - p.dim()) + tuple(p.shape))
+                if encoding.block_size is None and p.shape[1] != 1:
+                    raise NotImplementedError(f"a scale per input channel (shape {tuple(p.shape)}) cannot be packed")
+                return p.repeat_interleave(n // p.shape[0], 0)
+
+            int_scale = None
+            shared = getattr(encoding, "per_channel_scale", None)
+            if shared is not None and tuple(shared.shape) == (n, 1) and 2 ** (encoding.decompressed_bw - encoding.bitwidth) <= 255:
+                int_scale = encoding.per_block_int_scale
+                if not torch.equal(int_scale * shared, scale):  # keep exactly the scales that are simulated
+                    int_scale = None
+            if int_scale is not None:
+                return cls.from_codes(codes, shared, per_channel(offset), qmin=encoding.qmin, int_scale=int_scale)
+            return cls.from_codes(codes, per_channel(scale), per_channel(offset), qmin=encoding.qmin)
+
+    @classmethod
+    def from_quantizer(cls, weight: torch.Tensor, quantizer) -> "PackedInt4Weight":
+        """Pack ``weight`` on the grid of a calibrated 4-bit weight quantizer."""
+        encoding = quantizer.get_encodings()
+        if encoding is None:
+            raise RuntimeError("the quantizer has no encodings yet: calibrate it before packing its weight")
+        return cls.from_encoding(weight, encoding)
+
+
+def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:  # pylint: disable=redefined-builtin
+    """``input @ w.T + bias`` for a packed weight: ``[..., in_features] -> [..., out_features]``.
+
+    float32, float16 or bfloat16 activations; sums in float32, one rounding to ``input.dtype``.  For
+    inference: an input or bias that needs a gradient is refused (train through the quantizer instead).
+    """
+    if not input.is_cuda:
+        raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
+    code = _lib.DTYPE_CODE.get(input.dtype)
+    if code is None or code == _lib.AB_F64:
+        raise NotImplementedError(f"linear_int4 takes float32, float16 or bfloat16 activations, got {input.dtype}")
+    if input.dim() == 0 or input.shape[-1] != weight.in_features:
+        raise RuntimeError(f"expected {weight.in_features} input features, got an input of shape {tuple(input.shape)}")
+    if input.device != weight.device:
+        raise RuntimeError(f"input is on {input.device}, the weight on {weight.device}")
+    if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
+        raise RuntimeError("linear_int4 has no backward pass: call it under torch.no_grad(), or train through the weight's quantizer")
+    if bias is not None:
+        if bias.dtype != input.dtype or bias.device != input.device or tuple(bias.shape) != (weight.out_features,):
+            raise RuntimeError(f"bias must be {input.dtype} of shape {(weight.out_features,)} on {input.device}, "
+                               f"got {bias.dtype} of shape {tuple(bias.shape)} on {bias.device}")
+        bias = bias.contiguous()
+    out = torch.empty(input.shape[:-1] + (weight.out_features,), dtype=input.dtype, device=input.device)
+    tokens = math.prod(input.shape[:-1])
+    if tokens == 0:
+        return out
+    x = input.reshape(tokens, weight.in_features)
+    if x.stride(1) != 1 and weight.in_features > 1:
+        x = x.contiguous()
+    ldx = x.stride(0)
+    if tokens > 1 and ldx < weight.in_features:  # rows that overlap (an expanded input)
+        x = x.contiguous()
+        ldx = weight.in_features
+    with _lib.on_device(input.device):
+        check(lib.aimet_b200_int4_linear(weight._desc, x.data_ptr(), ldx, None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
+                                         weight.out_features, tokens, code, _lib.stream_ptr(input.device)))
+    return out

@@ -1,0 +1,225 @@
+"""A paged key / value cache held in 8 bits, and attention over it.
+
+:class:`Int8KVCache` keeps the keys and values of a decoder layer as signed 8-bit codes on a symmetric
+grid, one scale per page (a block of tokens) and head.  :meth:`Int8KVCache.append` quantizes new tokens
+into it, :meth:`Int8KVCache.attention` attends over it reading one byte per element, and
+:meth:`Int8KVCache.gather` reads tokens back as values.  Token ``j`` of a sequence lies in row
+``j % page_size`` of page ``block_table[sequence, j // page_size]``; which pages belong to whom is the
+caller's, lengths and tables stay on the device, nothing waits for the host, so a decode step can be
+captured into a CUDA graph.  Inference only: inputs that need a gradient are refused.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+
+__all__ = ["Int8KVCache"]
+
+_Strides = ctypes.c_int64 * 3
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+class Int8KVCache:
+    """``num_pages`` pages of ``page_size`` tokens for ``num_heads`` key / value heads of ``head_dim``.
+
+    ``key``, ``value``: int8 ``[num_pages, num_heads, page_size, head_dim]``, codes in [-127, 127];
+    ``key_scale``, ``value_scale``: float32 ``[num_pages, num_heads]``; a code stands for ``code * scale``.
+    ``page_size`` is a multiple of 16 up to 1024, ``head_dim`` a multiple of 16 up to 256.
+    """
+
+    def __init__(self, num_pages: int, num_heads: int, page_size: int, head_dim: int, device="cuda"):
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
+        self._check_sizes(num_pages, num_heads, page_size, head_dim)
+        shape = (num_pages, num_heads, page_size, head_dim)
+        self._adopt(torch.zeros(shape, dtype=torch.int8, device=device), torch.zeros(shape, dtype=torch.int8, device=device),
+                    torch.zeros(shape[:2], device=device), torch.zeros(shape[:2], device=device))
+
+    @classmethod
+    def from_buffers(cls, key: torch.Tensor, value: torch.Tensor, key_scale: torch.Tensor,
+                     value_scale: torch.Tensor) -> "Int8KVCache":
+        """A cache over existing buffers (used in place; shapes and dtypes as in the class)."""
+        if key.dim() != 4:
+            raise RuntimeError(f"key must be [num_pages, num_heads, page_size, head_dim], got shape {tuple(key.shape)}")
+        for name, t, dtype, shape in (("key", key, torch.int8, key.shape), ("value", value, torch.int8, key.shape),
+                                      ("key_scale", key_scale, torch.float32, key.shape[:2]),
+                                      ("value_scale", value_scale, torch.float32, key.shape[:2])):
+            if t.dtype != dtype or t.shape != shape or t.device != key.device:
+                raise RuntimeError(f"{name} must be {dtype} of shape {tuple(shape)} on {key.device}, got {t.dtype} of shape "
+                                   f"{tuple(t.shape)} on {t.device}")
+            if not t.is_contiguous():
+                raise RuntimeError(f"{name} must be contiguous")
+        cls._check_sizes(*key.shape)
+        if not key.is_cuda:
+            raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
+        if key.data_ptr() % 16 or value.data_ptr() % 16:
+            raise RuntimeError("key and value must be 16-byte aligned")
+        cache = cls.__new__(cls)
+        cache._adopt(key, value, key_scale, value_scale)
+        return cache
+
+    @staticmethod
+    def _check_sizes(num_pages, num_heads, page_size, head_dim):
+        if num_pages < 1 or num_heads < 1:
+            raise RuntimeError(f"a cache needs pages and heads, got num_pages={num_pages}, num_heads={num_heads}")
+        if num_heads > 1024:
+            raise NotImplementedError(f"num_heads={num_heads}: up to 1024 are supported")
+        if page_size < 16 or page_size % 16 or page_size > 1024:
+            raise NotImplementedError(f"page_size={page_size}: a multiple of 16 up to 1024 is supported")
+        if head_dim < 16 or head_dim % 16 or head_dim > 256:
+            raise NotImplementedError(f"head_dim={head_dim}: a multiple of 16 up to 256 is supported")
+
+    def _adopt(self, key, value, key_scale, value_scale):
+        self.key, self.value, self.key_scale, self.value_scale = key, value, key_scale, value_scale
+        self.num_pages, self.num_heads, self.page_size, self.head_dim = key.shape
+        self.device = key.device
+        self._desc = _lib.KVCache(key.data_ptr(), value.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(),
+                                  self.num_pages, self.num_heads, self.page_size, self.head_dim, 0)
+
+    def __repr__(self):
+        return (f"Int8KVCache(num_pages={self.num_pages}, num_heads={self.num_heads}, page_size={self.page_size}, "
+                f"head_dim={self.head_dim}, device={self.device})")
+
+    # ---- argument checks -------------------------------------------------------------------
+    def _tokens(self, t: torch.Tensor, name: str) -> int:
+        """Checks a [sequences, tokens, heads, head_dim] input; returns its dtype code."""
+        if not t.is_cuda:
+            raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
+        code = _lib.DTYPE_CODE.get(t.dtype)
+        if code is None or code == _lib.AB_F64:
+            raise NotImplementedError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+        if t.dim() != 4 or t.shape[3] != self.head_dim:
+            raise RuntimeError(f"{name} must be [sequences, tokens, heads, {self.head_dim}], got shape {tuple(t.shape)}")
+        if t.device != self.device:
+            raise RuntimeError(f"{name} is on {t.device}, the cache on {self.device}")
+        return code
+
+    def _table(self, table: torch.Tensor, seqs: int) -> torch.Tensor:
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != seqs or table.device != self.device:
+            raise RuntimeError(f"block_table must be int32 of shape ({seqs}, blocks) on {self.device}, got {table.dtype} of shape "
+                               f"{tuple(table.shape)} on {table.device}")
+        return table if table.stride(1) == 1 or table.shape[1] <= 1 else table.contiguous()
+
+    def _lens(self, lens: torch.Tensor, seqs: int, name: str) -> torch.Tensor:
+        if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != seqs or lens.device != self.device:
+            raise RuntimeError(f"{name} must be int32 of shape ({seqs},) on {self.device}, got {lens.dtype} of shape "
+                               f"{tuple(lens.shape)} on {lens.device}")
+        return lens if lens.is_contiguous() else lens.contiguous()
+
+    # ---- operators -------------------------------------------------------------------------
+    def append(self, key: torch.Tensor, value: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
+               new_lens: Optional[torch.Tensor] = None) -> None:
+        """Quantize new tokens into the cache.
+
+        ``key``, ``value``: ``[sequences, tokens, num_heads, head_dim]`` of one dtype, any strides;
+        ``context_lens``: int32 tokens that every sequence holds already; ``new_lens``: int32 tokens of
+        ``key`` / ``value`` that are real (default: all).  Token ``i`` becomes position ``context_lens + i``.
+
+        A block's scale is the largest magnitude of its tokens over 127.  While a partly filled block
+        takes in larger tokens its scale grows, by a quarter at least, and the codes it holds are rounded to
+        the new grid: a token ends within 2.5 steps of its value, within half a step if its block was
+        written at once.  NaN is stored as zero; infinities as the block's largest level, scales being taken
+        from finite values.  Tokens whose table entry is outside ``[0, num_pages)``, or lies behind the
+        table's end, are dropped.  Within a call no page may receive tokens of two sequences.
+        """
+        code = self._tokens(key, "key")
+        if value.dtype != key.dtype or value.shape != key.shape or value.device != key.device:
+            raise RuntimeError(f"value must be {key.dtype} of shape {tuple(key.shape)} on {key.device}, got {value.dtype} of shape "
+                               f"{tuple(value.shape)} on {value.device}")
+        if key.shape[2] != self.num_heads:
+            raise RuntimeError(f"key has {key.shape[2]} heads, the cache {self.num_heads}")
+        if _needs_grad(key, value):
+            raise RuntimeError("append has no backward pass: call it under torch.no_grad()")
+        seqs, tokens = key.shape[:2]
+        table = self._table(block_table, seqs)
+        context = self._lens(context_lens, seqs, "context_lens")
+        new = None if new_lens is None else self._lens(new_lens, seqs, "new_lens")
+        if key.stride(3) != 1:
+            key = key.contiguous()
+        if value.stride(3) != 1:
+            value = value.contiguous()
+        with _lib.on_device(self.device):
+            check(lib.aimet_b200_kv_append(
+                self._desc, key.data_ptr(), value.data_ptr(), _Strides(*key.stride()[:3]), _Strides(*value.stride()[:3]), seqs,
+                tokens, table.data_ptr(), table.stride(0), table.shape[1], context.data_ptr(), _lib.ptr(new), code,
+                _lib.stream_ptr(self.device)))
+
+    def gather(self, block_table: torch.Tensor, lens: torch.Tensor, length: Optional[int] = None,
+               dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Keys and values ``[sequences, length, num_heads, head_dim]`` of the first ``lens`` (int32) tokens
+        of every sequence, zeros behind; ``length`` defaults to all that the table can hold."""
+        code = _lib.DTYPE_CODE.get(dtype)
+        if code is None or code == _lib.AB_F64:
+            raise NotImplementedError(f"gather gives float32, float16 or bfloat16, not {dtype}")
+        seqs = block_table.shape[0] if block_table.dim() == 2 else -1
+        table = self._table(block_table, seqs)
+        lens = self._lens(lens, seqs, "lens")
+        if length is None:
+            length = table.shape[1] * self.page_size
+        if length < 0:
+            raise RuntimeError(f"length={length} is negative")
+        shape = (seqs, length, self.num_heads, self.head_dim)
+        key = torch.empty(shape, dtype=dtype, device=self.device)
+        value = torch.empty(shape, dtype=dtype, device=self.device)
+        if key.numel():
+            with _lib.on_device(self.device):
+                check(lib.aimet_b200_kv_gather(self._desc, key.data_ptr(), value.data_ptr(), seqs, length, table.data_ptr(),
+                                               table.stride(0), table.shape[1], lens.data_ptr(), code, _lib.stream_ptr(self.device)))
+        return key, value
+
+    def attention(self, query: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
+                  query_lens: Optional[torch.Tensor] = None, *, causal: bool = True, window: Optional[int] = None,
+                  scale: Optional[float] = None, return_lse: bool = False):
+        """Softmax attention of every sequence's newest tokens over its tokens in the cache.
+
+        ``query``: ``[sequences, tokens, heads, head_dim]``, any strides, ``heads`` a multiple of the
+        cache's (consecutive query heads share a cache head); ``context_lens``: int32 tokens in the cache,
+        the newest included (append first); ``query_lens``: int32 tokens of ``query`` that are real
+        (default: all).  Query ``i`` stands at position ``context_lens - query_lens + i`` and sees positions
+        up to its own (``causal``) and after its own minus ``window``; ``scale`` defaults to
+        ``head_dim ** -0.5``.  Scores, softmax and sums are float32.
+
+        Returns ``[sequences, tokens, heads, head_dim]`` in ``query.dtype``; queries that see nothing, and
+        those behind ``query_lens``, give zeros.  With ``return_lse`` also the logarithm of each query's
+        softmax sum, float32 ``[sequences, tokens, heads]`` (-inf where it sees nothing), by which results
+        over parts of a context can be joined.
+        """
+        code = self._tokens(query, "query")
+        if _needs_grad(query):
+            raise RuntimeError("attention over the cache has no backward pass: call it under torch.no_grad()")
+        seqs, tokens, heads = query.shape[:3]
+        if heads < 1 or heads % self.num_heads:
+            raise RuntimeError(f"{heads} query heads are no multiple of the cache's {self.num_heads}")
+        if window is not None and window < 1:
+            raise RuntimeError(f"window={window}: at least 1, or None for no window")
+        table = self._table(block_table, seqs)
+        context = self._lens(context_lens, seqs, "context_lens")
+        new = None if query_lens is None else self._lens(query_lens, seqs, "query_lens")
+        if query.stride(3) != 1:
+            query = query.contiguous()
+        out = torch.empty((seqs, tokens, heads, self.head_dim), dtype=query.dtype, device=self.device)
+        lse = torch.empty((seqs, tokens, heads), dtype=torch.float32, device=self.device) if return_lse else None
+        if out.numel():
+            group, width = heads // self.num_heads, table.shape[1]
+            with _lib.on_device(self.device):
+                need = lib.aimet_b200_kv_attention_scratch_bytes(self._desc, seqs, tokens, group, width, code)
+                check(need)
+                # from the caching allocator, call by call: buffers of two streams, or of two captured graphs,
+                # are never shared
+                part = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+                check(lib.aimet_b200_kv_attention(
+                    self._desc, query.data_ptr(), _Strides(*query.stride()[:3]), out.data_ptr(), _lib.ptr(lse), seqs, tokens, group,
+                    table.data_ptr(), table.stride(0), width, context.data_ptr(), _lib.ptr(new), int(causal), window or 0,
+                    self.head_dim ** -0.5 if scale is None else float(scale), code, _lib.ptr(part), need,
+                    _lib.stream_ptr(self.device)))
+        return (out, lse) if return_lse else out

@@ -18,6 +18,7 @@ import torch
 from torch import nn
 
 from .encoding_analyzer import MinMaxEncodingAnalyzer
+from .int4 import PackedInt4Weight, linear_int4
 from .quantizer import QuantizeDequantize
 
 __all__ = ["QuantizedLayer", "quantize_model", "compute_encodings", "quantized_layers", "precomputed"]
@@ -51,6 +52,10 @@ class QuantizedLayer(nn.Module):
         qi, qo, qw = self.input_quantizers[0], self.output_quantizers[0], self.param_quantizers["weight"]
         if qi is not None:
             x = qi(x)
+        packed = self.__dict__.get("_packed_weight")
+        if packed is not None and not torch.is_grad_enabled() and getattr(qw, "_observer_hook", None) is None:
+            out = linear_int4(x, packed, self.layer.bias)
+            return out if qo is None else qo(out)
         w = self.layer.weight if qw is None else self._quantized_weight(qw)
         if isinstance(self.layer, nn.Conv2d):
             out = self.layer._conv_forward(x, w, self.layer.bias)  # pylint: disable=protected-access
@@ -181,14 +186,26 @@ def _allreduce_minmax_statistics(quantizers, group):
             continue  # no rank observed this quantizer
         o.stats = _MinMaxRange(mn.to(dtype).reshape(o.shape), mx.to(dtype).reshape(o.shape))
 
+
+def _packable(layer: QuantizedLayer) -> bool:
+    """A Linear layer whose weight quantizer has a grid of at most 4 bits that the packed layout can hold."""
+    qw = layer.param_quantizers["weight"]
+    return isinstance(layer.layer, nn.Linear) and qw is not None and qw.is_initialized() and qw.qmax - qw.qmin <= 15
+
+
 @contextlib.contextmanager
-def precomputed(model: nn.Module):
+def precomputed(model: nn.Module, packed: bool = False):
     """Inference with frozen parameters: inside the context every quantizer derives its scale and
     offset once (the reference's ``_precompute_encodings``, quantizer.py:790-804, entered for a whole
     model as in aimet_torch/utils.py:1666) and every layer quantizes its weight once instead of on
     every forward (what the reference's ``fold_param_quantizers`` achieves, nn/base.py:1103-1155,
     without giving up the quantizers).  Nothing is cached outside the context, so weights and
-    ranges may be edited freely (in place, through ``.data``, by re-assignment) between contexts."""
+    ranges may be edited freely (in place, through ``.data``, by re-assignment) between contexts.
+
+    ``packed``: Linear layers with weights of at most 4 bits hold their codes packed
+    (:class:`aimet_b200.int4.PackedInt4Weight`) instead of the quantize-dequantized weight, a quarter of
+    its bytes in 16 bits, and multiply with them directly in no-grad forwards.  Grids that cannot be
+    packed, and layers of other kinds, are held as without ``packed``."""
     from .quantizer import derive_encodings
 
     with contextlib.ExitStack() as stack, torch.no_grad():
@@ -200,6 +217,12 @@ def precomputed(model: nn.Module):
             stack.enter_context(q._set_encodings(enc))  # pylint: disable=protected-access
         for layer in layers:
             qw = layer.param_quantizers["weight"]
+            if packed and _packable(layer):
+                try:
+                    layer.__dict__["_packed_weight"] = PackedInt4Weight.from_quantizer(layer.layer.weight, qw)
+                    continue
+                except NotImplementedError:
+                    pass
             if qw is not None and qw.is_initialized():
                 layer.__dict__["_held_weight"] = qw(layer.layer.weight).detach()
         try:
@@ -207,3 +230,4 @@ def precomputed(model: nn.Module):
         finally:
             for layer in layers:
                 layer.__dict__.pop("_held_weight", None)
+                layer.__dict__.pop("_packed_weight", None)

@@ -386,6 +386,84 @@ int aimet_b200_seqmse_linear_loss(const void *x, const void *xq, const void *w, 
  * a host check the give-up path of the SeqMSE kernel's waits without provoking any fault. */
 int aimet_b200_seqmse_wait_selftest(int32_t *status, int64_t limit_us, void *stream);
 
+/* ------------------------------------------------------------------------- *
+ * Products with 4-bit weights.  No counterpart in the reference, which only simulates
+ * quantized weights; the grids are the ones its weight quantizers calibrate
+ * (quantization/affine/quantizer.py:1072-1440):
+ *   w[i][j] = (code[i][j] + offset[i][g]) * scale[i][g],  code in [qmin, qmin + 15]
+ * codes: aimet_b200_int4_codes_bytes() bytes written by aimet_b200_int4_pack (u = code - qmin).
+ * scales, zeros: one entry per channel and block, stored as
+ *   [ceil(n / 16)][ceil(tiles / per)][16][sub],  tiles = ceil(k / 64), per = max(1, block / 64),
+ *   sub = max(1, 64 / block): entry [i / 16][..][i % 16][..] belongs to channel i, zeros in what
+ *   lies behind the matrix.
+ * scale_kind 0: scales are float32.  scale_kind 1: scales are uint8 factors of row_scale[channel]
+ * (float32, one per channel): the blockwise grid of GroupedBlockQuantizeDequantize.
+ * zeros: int8, z = -(qmin + offset) per channel and block, |z| <= 112 (what 16-bit floats subtract
+ * exactly); NULL: `zero` for all.
+ * ------------------------------------------------------------------------- */
+typedef struct ab_int4_weight {
+    int64_t n, k;       /* output channels, input channels */
+    int32_t block;      /* input channels per scale: 16, 32 or a multiple of 64 */
+    int32_t scale_kind; /* 0 float32, 1 uint8 factors of row_scale */
+    int32_t zero;       /* zero point where zeros is NULL */
+    int32_t reserved;
+    const void *codes, *scales, *zeros, *row_scale;
+} ab_int4_weight;
+
+int64_t aimet_b200_int4_codes_bytes(int64_t n, int64_t k);
+/* codes: int8 [n][k], each in [qmin, qmin + 15] (the four low bits of code - qmin are kept) */
+int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int qmin, void *out, void *stream);
+/* y[m][i] = sum_j x[m][j] * w[i][j] + bias[i] for `tokens` rows; x rows are ldx elements apart, y rows
+ * ldy; bias (io_dtype, n elements) may be NULL.  Float32 accumulation, one rounding to io_dtype. */
+int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *x, int64_t ldx, const void *bias, void *y,
+                           int64_t ldy, int64_t tokens, int io_dtype, void *stream);
+
+/* ------------------------------------------------------------------------- *
+ * A paged key / value cache in 8-bit codes and attention over it.  No counterpart in the
+ * reference.  value of a code = code * scale, one scale per page (a block of page_size tokens)
+ * and head:
+ *   key, value              int8 [num_pages][num_heads][page_size][head_dim], 16-byte aligned
+ *   key_scale, value_scale  float32 [num_pages][num_heads]
+ * Token j of sequence s lives in row j % page_size of page block_table[s][j / page_size]
+ * (int32, rows table_stride apart, table_width entries).  Entries outside [0, num_pages) mean "no
+ * page": nothing is written there, reads give zeros, attention masks the tokens.  page_size is a
+ * multiple of 16 up to 1024, head_dim a multiple of 16 up to 256.  strides: elements between
+ * sequences, tokens and heads (the last dim is contiguous).
+ * ------------------------------------------------------------------------- */
+typedef struct ab_kv_cache {
+    void *key, *value, *key_scale, *value_scale;
+    int64_t num_pages;
+    int32_t num_heads, page_size, head_dim, reserved;
+} ab_kv_cache;
+
+/* Tokens [0, new_lens[s]) of key / value [seqs][tokens][num_heads][head_dim] become positions
+ * context_lens[s] .. of sequence s (new_lens NULL: all).  Block by block: a block that starts with
+ * a new token gets scale = max|x| / 127 over its new tokens' finite values; a partly filled one keeps
+ * its scale if that is at least max|x| / 127 and else gets max(max|x| / 127, 1.25 * scale), the codes in
+ * it becoming rint(code * (old / new)).  code = clamp(rint(x / scale), -127, 127); NaN is stored as
+ * zero.  Two sequences of a call must not append into the same page. */
+int aimet_b200_kv_append(const ab_kv_cache *cache, const void *key, const void *value, const int64_t *key_strides,
+                         const int64_t *value_strides, int64_t seqs, int64_t tokens, const int32_t *block_table,
+                         int64_t table_stride, int64_t table_width, const int32_t *context_lens,
+                         const int32_t *new_lens, int io_dtype, void *stream);
+/* key, value [seqs][length][num_heads][head_dim]: the values at positions [0, lens[s]), zeros behind */
+int aimet_b200_kv_gather(const ab_kv_cache *cache, void *key, void *value, int64_t seqs, int64_t length,
+                         const int32_t *block_table, int64_t table_stride, int64_t table_width, const int32_t *lens,
+                         int io_dtype, void *stream);
+/* out[s][i][h] = sum_j softmax_j(softmax_scale * query . key_j) value_j over the tokens j of sequence s,
+ * j < context_lens[s] (which counts the newest tokens); query [seqs][tokens][num_heads * group][head_dim],
+ * head h reads head h / group of the cache.  Query i < query_lens[s] (NULL: all) stands at position
+ * p = context_lens[s] - query_lens[s] + i; causal != 0: j <= p; window > 0: j > p - window.  Rows that see
+ * nothing, and rows behind query_lens[s], are zero.  lse (float32 [seqs][tokens][num_heads * group], may be
+ * NULL): log of the sum of exp(score), -infinity for those rows. */
+int64_t aimet_b200_kv_attention_scratch_bytes(const ab_kv_cache *cache, int64_t seqs, int64_t tokens, int64_t group,
+                                              int64_t table_width, int io_dtype);
+int aimet_b200_kv_attention(const ab_kv_cache *cache, const void *query, const int64_t *query_strides, void *out,
+                            float *lse, int64_t seqs, int64_t tokens, int64_t group, const int32_t *block_table,
+                            int64_t table_stride, int64_t table_width, const int32_t *context_lens,
+                            const int32_t *query_lens, int causal, int64_t window, double softmax_scale, int io_dtype,
+                            void *scratch, int64_t scratch_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

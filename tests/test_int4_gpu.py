@@ -1,0 +1,297 @@
+"""Products with packed 4-bit weights against the same product in 64 bits.
+
+Tolerance, element by element, with S = sum |x| |w|: the result is rounded once to the output type (at most
+eps / 2 of it); float32 sums take at most k / 16 + 32 additions in a row, each off by at most 2^-23 of S (a
+tensor core may truncate); the scale's and the multiplier's own roundings are inside that count.  A weight that
+is rounded to 16 bits before the product (many tokens) adds eps / 2 of S.
+"""
+
+import pytest
+import torch
+from torch import nn
+
+pytestmark = pytest.mark.gpu
+
+
+def make(n, k, block, grid, seed=0, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    blocks = k // (block or k)
+    qmin = 0 if grid == "asym" else -8
+    codes = torch.randint(qmin, qmin + 16, (n, k), generator=g).to(torch.int8)
+    scale = torch.rand(n, blocks, generator=g) * 0.1 + 0.01
+    offset = -torch.randint(0, 16, (n, blocks), generator=g).float() if grid == "asym" else None
+    int_scale = None
+    if grid == "lpbq":
+        int_scale = torch.randint(1, 17, (n, blocks), generator=g).to(torch.uint8)
+        scale = scale[:, :1].contiguous()
+    dev = lambda t: None if t is None else t.to(device)  # noqa: E731
+    return dev(codes), dev(scale), dev(offset), qmin, dev(int_scale)
+
+
+def dequantized(codes, scale, offset, int_scale):
+    n, k = codes.shape
+    s = scale.double() if int_scale is None else scale.double() * int_scale.double()
+    block = k // s.shape[1]
+    w = codes.double()
+    if offset is not None:
+        w = w + offset.double().repeat_interleave(block, 1)
+    return w * s.repeat_interleave(block, 1)
+
+
+def packed_of(codes, scale, offset, qmin, int_scale):
+    from aimet_b200.int4 import PackedInt4Weight
+
+    return PackedInt4Weight.from_codes(codes, scale, offset, qmin=qmin, int_scale=int_scale)
+
+
+def assert_close(got, x, w, bias=None, weight_in_16=False):
+    xd = x.double().reshape(-1, x.shape[-1])
+    want = xd @ w.T
+    size = xd.abs() @ w.abs().T
+    if bias is not None:
+        want, size = want + bias.double(), size + bias.double().abs()
+    half = torch.finfo(got.dtype).eps / 2
+    steps = w.shape[1] / 16 + 32
+    bound = half * want.abs() + steps * 2.0**-23 * size * (1 + half)
+    if weight_in_16:
+        bound = bound + half * size * (1 + half)
+    if got.dtype == torch.float16:
+        bound = bound + 2.0**-25  # below float16's smallest normal number the step no longer shrinks
+    err = (got.double().reshape(want.shape) - want).abs()
+    assert bool((err <= bound).all()), f"off by {float((err / bound).max()):.3g} bounds at {int((err / bound).argmax())}"
+
+
+# tokens from one to several tiles, channels and columns that fit no tile, blocks from 16 to the row
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("grid", ["sym", "asym", "lpbq"])
+@pytest.mark.parametrize("tokens,n,k,block", [
+    (1, 16, 64, 64), (1, 1, 16, 16), (1, 33, 128, 16), (3, 40, 96, 32), (8, 17, 320, 64), (9, 64, 640, 128), (16, 200, 1024, 256),
+    (2, 100, 1040, 16), (5, 48, 144, 48), (7, 31, 480, 96), (4, 24, 1, 0), (1, 50, 77, 0), (3, 65, 1001, 0), (17, 130, 2080, 32),
+])
+def test_matches_the_product_in_64_bits(dtype, grid, tokens, n, k, block):
+    from aimet_b200.int4 import linear_int4
+
+    parts = make(n, k, block, grid, seed=n + k)
+    codes, scale, offset, _, int_scale = parts
+    g = torch.Generator().manual_seed(tokens)
+    x = torch.randn(tokens, k, generator=g).to(dtype).cuda()
+    bias = torch.randn(n, generator=g).to(dtype).cuda() if tokens % 2 else None
+    got = linear_int4(x, packed_of(*parts), bias)
+    assert got.shape == (tokens, n) and got.dtype == dtype
+    assert_close(got, x, dequantized(codes, scale, offset, int_scale), bias, weight_in_16=tokens > 16 and dtype != torch.float32)
+
+
+# many tokens: whole tiles and ragged ones, odd columns, every block class
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("grid,tokens,n,k,block", [
+    ("sym", 64, 256, 512, 128), ("asym", 129, 300, 1024, 64), ("lpbq", 257, 130, 768, 32), ("asym", 40, 513, 272, 16),
+    ("sym", 100, 128, 333, 0), ("asym", 515, 640, 4096, 128), ("lpbq", 33, 1000, 2048, 256), ("sym", 300, 72, 64, 64),
+])
+def test_many_tokens(dtype, grid, tokens, n, k, block):
+    from aimet_b200.int4 import linear_int4
+
+    parts = make(n, k, block, grid, seed=tokens)
+    codes, scale, offset, _, int_scale = parts
+    x = torch.randn(tokens, k, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    got = linear_int4(x, packed_of(*parts), bias)
+    assert_close(got, x, dequantized(codes, scale, offset, int_scale), bias, weight_in_16=dtype != torch.float32)
+
+
+@pytest.mark.parametrize("tokens", [3, 70])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_strides_alignment_and_leading_dims(dtype, tokens):
+    from aimet_b200.int4 import linear_int4
+
+    parts = make(48, 256, 64, "asym")
+    w, p = dequantized(*[parts[i] for i in (0, 1, 2, 4)]), packed_of(*parts)
+    base = torch.randn(tokens, 600, device="cuda").to(dtype)
+    for x in (base[:, :256], base[:, 1:257], base[:, 3:259], base.t()[:256].t().contiguous().t().contiguous().t(),
+              base[:1, :256].expand(tokens, 256), base[::2, 8:264]):
+        assert_close(linear_int4(x, p), x, w, weight_in_16=x.shape[0] > 16 and dtype != torch.float32)
+    x = base[:2, :512].reshape(2, 2, 256)
+    assert linear_int4(x, p).shape == (2, 2, 48)
+    assert_close(linear_int4(x, p), x, w)
+    assert linear_int4(base[0, :256], p).shape == (48,)
+    assert linear_int4(base[:0, :256], p).shape == (0, 48)
+
+
+def test_float32_values_over_the_whole_range():
+    """A float32 activation is cut into terms; large, small and infinite values and NaN survive that."""
+    from aimet_b200.int4 import linear_int4
+
+    codes, scale, offset, qmin, _ = make(32, 64, 64, "sym")
+    scale = torch.full_like(scale, 2.0**-10)
+    w, p = dequantized(codes, scale, None, None), packed_of(codes, scale, None, qmin, None)
+    g = torch.Generator().manual_seed(5)
+    x = (torch.randn(6, 64, generator=g) * torch.tensor([1e36, 1e-30, 1.0, 1e30, 3e-20, 1e10])[:, None]).cuda()
+    x[0] = x[0].clamp(-1e36, 1e36)
+    assert_close(linear_int4(x, p), x, w)
+    big = torch.zeros(1, 64, device="cuda")
+    big[0, 3] = torch.finfo(torch.float32).max  # rounds up past bfloat16's largest value
+    assert_close(linear_int4(big, p), big, w)
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        y = x.clone()
+        y[2, 5] = bad
+        got, want = linear_int4(y, p), y.float() @ w.float().T
+        assert torch.equal(torch.isnan(got[2]), torch.isnan(want[2])) and torch.equal(torch.isinf(got[2]), torch.isinf(want[2]))
+        assert_close(got[3:], y[3:], w)
+
+
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_rows_keep_to_themselves(tokens):
+    """A row's result does not depend on what else is in the call, and two calls agree to the bit."""
+    from aimet_b200.int4 import linear_int4
+
+    parts = make(100, 512, 64, "asym")
+    p = packed_of(*parts)
+    x = torch.randn(tokens, 512, device="cuda").bfloat16()
+    one = linear_int4(x, p)
+    assert torch.equal(one, linear_int4(x, p))
+    y = x.clone()
+    y[-1] = float("nan")
+    assert torch.equal(linear_int4(y, p)[:-1], one[:-1])
+
+
+def test_calls_captured_into_graphs_and_on_other_streams():
+    from aimet_b200.int4 import linear_int4
+
+    parts = make(256, 512, 64, "lpbq")
+    w, p = dequantized(*[parts[i] for i in (0, 1, 2, 4)]), packed_of(*parts)
+    graphs, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i, tokens in enumerate((2, 50)):
+        x = torch.randn(tokens, 512, device="cuda").half()
+        linear_int4(x, p)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[i]):
+            y = linear_int4(x, p)
+        graphs.append((graph, x, y))
+    for _ in range(3):
+        for _, x, _ in graphs:
+            x.normal_()
+        torch.cuda.synchronize()
+        for i, (graph, _, _) in enumerate(graphs):
+            with torch.cuda.stream(streams[i]):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, x, y in graphs:
+            assert_close(y, x, w, weight_in_16=True)
+
+
+@pytest.mark.parametrize("kind", ["per_tensor", "per_channel", "blockwise", "asymmetric", "lpbq", "int3"])
+def test_packs_what_the_quantizers_calibrate(kind):
+    from aimet_b200.int4 import PackedInt4Weight, linear_int4
+    from aimet_b200.quantizer import GroupedBlockQuantizeDequantize, QuantizeDequantize
+
+    torch.manual_seed(0)
+    weight = (torch.randn(96, 256) * torch.rand(96, 1)).cuda()
+    if kind == "lpbq":
+        q = GroupedBlockQuantizeDequantize((96, 4), 4, True, 8, block_size=(1, 64), block_grouping=(1, 4))
+    else:
+        shape, block = {"per_tensor": ((), None), "per_channel": ((96, 1), None)}.get(kind, ((96, 8), (1, 32)))
+        q = QuantizeDequantize(shape, 3 if kind == "int3" else 4, kind != "asymmetric", block_size=block)
+    q = q.cuda()
+    with q.compute_encodings():
+        q(weight)
+    p = PackedInt4Weight.from_quantizer(weight, q)
+    # float32 simulation rounds (code + offset) * scale once more: half a step of each weight
+    x = torch.randn(4, 256, device="cuda")
+    with torch.no_grad():
+        w = q(weight).double()
+        got = linear_int4(x, p).double()
+    size = x.double().abs() @ w.abs().T
+    assert bool(((got - x.double() @ w.T).abs() <= (256 / 16 + 32 + 4) * 2.0**-23 * size).all())
+    assert p.nbytes < weight.numel() * 4 / 4
+    if kind == "lpbq":
+        assert p._desc.scale_kind == 1  # the integer factors are kept as bytes
+
+
+def test_model_with_packed_weights():
+    """nn.precomputed(model, packed=True): same results as the simulated weights up to the sums' rounding."""
+    from aimet_b200 import nn as qnn
+
+    torch.manual_seed(0)
+    model = nn.Sequential(nn.Linear(64, 96), nn.ReLU(), nn.Linear(96, 40, bias=False)).cuda().eval()
+    qnn.quantize_model(model, param_bw=4, act_bw=16)
+    x = torch.randn(7, 64, device="cuda")
+    with torch.no_grad(), qnn.compute_encodings(model):
+        model(x)
+    layers = list(qnn.quantized_layers(model))
+    with torch.no_grad():
+        with qnn.precomputed(model):
+            want = model(x)
+        with qnn.precomputed(model, packed=True):
+            assert all("_packed_weight" in layer.__dict__ and "_held_weight" not in layer.__dict__ for layer in layers)
+            got = model(x)
+        # 16-bit activation grids: a sum off by its rounding may land one step further (2^-16 of the range),
+        # and the second layer multiplies such steps of its 96 inputs
+        out_range = float(want.max() - want.min())
+        hidden = layers[1].input_quantizers[0]
+        step_in = float((hidden.get_max() - hidden.get_min()) / 65535)
+        w = layers[1].param_quantizers["weight"](layers[1].layer.weight)
+        bound = float(w.abs().sum(1).max()) * step_in * 2 + 2 * out_range / 65535
+        assert float((got - want).abs().max()) <= bound
+        assert all("_packed_weight" not in layer.__dict__ for layer in layers)
+        assert torch.equal(model(x), want)
+    with qnn.precomputed(model, packed=True), torch.enable_grad():  # gradients: the simulated weight is used
+        y = model(x.requires_grad_(True))
+        y.sum().backward()
+        assert x.grad is not None and layers[0].layer.weight.grad is not None
+    # an 8-bit weight is held as before
+    model8 = qnn.quantize_model(nn.Sequential(nn.Linear(64, 8)).cuda(), param_bw=8)
+    with torch.no_grad(), qnn.compute_encodings(model8):
+        model8(x)
+    with torch.no_grad(), qnn.precomputed(model8, packed=True):
+        assert "_held_weight" in model8[0].__dict__ and "_packed_weight" not in model8[0].__dict__
+
+
+def test_refusals():
+    from aimet_b200.int4 import PackedInt4Weight, linear_int4
+
+    codes, scale, offset, qmin, _ = make(16, 64, 32, "asym")
+    p = packed_of(codes, scale, offset, qmin, None)
+    x = torch.randn(2, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        linear_int4(x.clone().requires_grad_(True), p)
+    with pytest.raises(RuntimeError, match="input features"):
+        linear_int4(x[:, :32], p)
+    with pytest.raises(RuntimeError, match="bias must be"):
+        linear_int4(x, p, torch.zeros(17, device="cuda"))
+    with pytest.raises(RuntimeError, match="bias must be"):
+        linear_int4(x, p, torch.zeros(16, device="cuda", dtype=torch.half))
+    with pytest.raises(NotImplementedError, match="float64"):
+        linear_int4(x.double(), p)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        linear_int4(x.cpu(), p)
+    with pytest.raises(RuntimeError, match="whole numbers"):
+        PackedInt4Weight.from_codes(codes.float() + 0.5, scale, offset, qmin=0)
+    with pytest.raises(RuntimeError, match="whole numbers"):
+        PackedInt4Weight.from_codes(codes, scale, offset, qmin=1)
+    with pytest.raises(RuntimeError, match="do not divide"):
+        PackedInt4Weight.from_codes(codes, scale[:8], None, qmin=0)
+    with pytest.raises(RuntimeError, match="do not divide"):
+        PackedInt4Weight.from_codes(codes[:, :63], scale, None, qmin=0)
+    with pytest.raises(NotImplementedError, match="multiple of 16"):
+        PackedInt4Weight.from_codes(codes, torch.ones(16, 8, device="cuda"), None, qmin=0)
+    with pytest.raises(NotImplementedError, match="whole numbers"):
+        PackedInt4Weight.from_codes(codes, scale, offset + 0.5, qmin=0)
+    with pytest.raises(NotImplementedError, match="112"):
+        PackedInt4Weight.from_codes(codes, scale, offset - 200, qmin=0)
+    with pytest.raises(RuntimeError, match="int_scale"):
+        PackedInt4Weight.from_codes(codes, scale[:, :1].contiguous(), None, qmin=0, int_scale=torch.full((16, 2), 300, device="cuda"))
+    with pytest.raises(RuntimeError, match="non-empty"):
+        PackedInt4Weight.from_codes(codes[:0], scale[:0], None, qmin=0)
+
+
+def test_zero_points_beyond_the_grid():
+    """Offsets need not lie on the grid: every whole zero point up to 112 is subtracted exactly."""
+    from aimet_b200.int4 import linear_int4
+
+    codes, scale, _, _, _ = make(32, 128, 32, "asym")
+    offset = torch.randint(-112, 113, scale.shape, device="cuda").float()
+    offset[0, 0], offset[1, 1] = 112.0, -112.0
+    w, p = dequantized(codes, scale, offset, None), packed_of(codes, scale, offset, 0, None)
+    for dtype in (torch.bfloat16, torch.float16, torch.float32):
+        x = torch.randn(3, 128, device="cuda").to(dtype)
+        assert_close(linear_int4(x, p), x, w)
