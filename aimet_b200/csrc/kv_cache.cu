@@ -29,9 +29,9 @@ __host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b 
 // append
 //
 // One CTA per (sequence, touched block, head, key or value): largest magnitude of the block's new
-// tokens, the block's scale, codes.  A block that starts with a new token takes scale = max / 127; one
-// that holds tokens already keeps its scale while that covers the new tokens and otherwise takes
-// max(max / 127, 1.25 * scale), its codes becoming rint(code * (old / new)).  Growing by a quarter at
+// tokens, the block's scale, codes.  A block that starts with a new token takes scale = max * (1 / 127),
+// the factor rounded to float32 (what torch computes for max / 127 on a GPU); one that holds tokens
+// already keeps its scale while that covers the new tokens and otherwise takes max(that, 1.25 * scale), its codes becoming rint(code * (old / new)).  Growing by a quarter at
 // least bounds what repeated rounding can add up to: half a step each time, 2.5 final steps in all.
 //
 // Bound by reading the new tokens and writing a byte for each element.  x / scale is the correctly rounded
@@ -129,7 +129,7 @@ template <typename E, int THREADS> __global__ void __launch_bounds__(THREADS) k_
     }
 
     const float old = kept ? *scale_at : 0.f;
-    float scale = __fdiv_rn(top, kLevels);
+    float scale = __fmul_rn(top, 1.f / kLevels);
     if (kept) scale = scale <= old ? old : fmaxf(scale, __fmul_rn(old, kGrowth));
     if (THREADS > 32)
         __syncthreads();  // everyone has read the old scale

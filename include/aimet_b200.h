@@ -438,8 +438,8 @@ typedef struct ab_kv_cache {
 
 /* Tokens [0, new_lens[s]) of key / value [seqs][tokens][num_heads][head_dim] become positions
  * context_lens[s] .. of sequence s (new_lens NULL: all).  Block by block: a block that starts with
- * a new token gets scale = max|x| / 127 over its new tokens' finite values; a partly filled one keeps
- * its scale if that is at least max|x| / 127 and else gets max(max|x| / 127, 1.25 * scale), the codes in
+ * a new token gets scale = max|x| * float32(1 / 127) over its new tokens' finite values; a partly filled
+ * one keeps its scale if that is at least as large and else gets max(max|x| * float32(1 / 127), 1.25 * scale), the codes in
  * it becoming rint(code * (old / new)).  code = clamp(rint(x / scale), -127, 127); NaN is stored as
  * zero.  Two sequences of a call must not append into the same page. */
 int aimet_b200_kv_append(const ab_kv_cache *cache, const void *key, const void *value, const int64_t *key_strides,

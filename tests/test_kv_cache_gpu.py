@@ -1,6 +1,6 @@
 """The 8-bit key / value cache: what append writes, what gather reads, attention over it.
 
-append: the scale is float32(max / 127), a code the nearest whole number to x / scale; the quotient is rounded
+append: the scale is max * float32(1 / 127) in float32, a code the nearest whole number to x / scale; the quotient is rounded
 to float32 before that, which moves it by at most 127 * 2^-24, so |code - x / scale| <= 1/2 + 127 * 2^-24
 (and 127 * 2^-22 where a held code is multiplied by a rounded ratio).
 
@@ -282,7 +282,7 @@ def expected_append(cache, key, value, table, context, new):
                 for name, x in (("key", key), ("value", value)):
                     t = x[s, lo - start:hi - start].double().transpose(0, 1)
                     finite = torch.where(torch.isfinite(t), t, 0.0)
-                    want = (finite.abs().amax((1, 2)) / LEVELS).float()
+                    want = finite.abs().amax((1, 2)).float() * torch.tensor(1 / LEVELS, device="cuda")
                     old = before[name + "_scale"][p]
                     if kept:
                         want = torch.where(want <= old, old, torch.maximum(want, (old.double() * 1.25).float()))
