@@ -8,40 +8,46 @@
 // float32 would take more instructions than it can issue.  So pairs of codes are turned into pairs of
 // 16-bit floats (a shift and one three-input logic operation put the code into the mantissa of 128
 // (bfloat16) or 1024 (float16); subtracting 128 + z or 1024 + z is exact) and multiplied 16 x 8 x 16
-// at a time by mma.sync with the weights as the 16-row operand and up to eight tokens as the 8 columns.
+// at a time by mma.sync with the weights as the 16-row operand and up to eight tokens as the 8 columns
+// (tcgen05 has 64 rows at least, and the tensor cores are 12 % busy as it is).
 // Products of a 16-bit activation with an integer below 2^8 are exact, sums are float32; every 64
 // columns (or smaller blocks) the sums are multiplied by the block's scale and added up in float32.
 // A float32 activation is cut into three bfloat16 terms that together hold all its 24 bits, each
 // multiplied by the same weights into the same sums.
 //
 // Layout of the codes: tiles of 16 channels x 64 columns, 512 bytes, one 16-byte load per lane; the
-// 32 codes of a lane are the operand fragments of four MMAs.  Columns are permuted within groups of 16
-// so that the matching fragment of x is one 8-byte load: lane t of a quad holds columns 4t .. 4t+3.
+// 32 codes of a lane are the operand fragments of four MMAs.  Columns are permuted within groups of 32
+// so that the matching fragment of x is one 16-byte read: lane t of a quad holds eight neighbouring
+// columns of every 32 (with blocks of 16 columns, four of every 16).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 
 namespace ab {
 namespace {
 
-constexpr int kTileN = 16;   // output channels per tile
-constexpr int kTileK = 64;   // input channels per tile
-constexpr int kMvWarps = 8;  // warps of a matvec CTA, each with a share of the columns
-constexpr int kMvDepth = 4;  // tiles requested ahead by a warp
+constexpr int kTileN = 16;    // output channels per tile
+constexpr int kTileK = 64;    // input channels per tile
+constexpr int kChunkK = 256;  // input channels per chunk: four tiles, 2 KB that one warp requests at once
+constexpr int kMvWarps = 8;   // warps of a matvec CTA
+constexpr int kMvTiles = kMvWarps;  // channel tiles of a CTA: at most as many as warps, so that a warp meets two at most
+constexpr int64_t kMaxK = 1ll << 20;
 
 __host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// scales, multipliers and zero points: one entry per channel and block, four, two or one blocks of a
-// 64-column tile side by side, [channel tile][tile of columns (or wider block)][16][sub]
+// Codes [channel tile][tile of columns][lane][16 bytes]; scales (float32, or uint8 factors) and zero points
+// (int8) [channel tile][chunk][entry][channel][sub]: one entry per chunk (blocks of 256 columns or more), two
+// (128) or four (64 or fewer, with 64 / block neighbouring blocks in an entry).  What lies behind the matrix
+// is there and multiplies zeros of x.
 struct Int4View {
     const uint4 *codes;
     const void *scales;
-    const int8_t *zeros;      // NULL: `zero` for all
-    const float *row_scale;   // scale kind 1
+    const int8_t *zeros;  // NULL: `zero` for all
+    const float *row_scale;
     int64_t n, k;
-    int kt;                   // tiles along k
-    int per;                  // tiles of columns that share a block (1 for blocks of up to 64)
-    int entries;              // entries along k: div_up(kt, per)
+    int chunks;   // per row: div_up(k, kChunkK)
+    int entries;  // per chunk: 1, 2, 4
     float zero;
 };
 
@@ -63,9 +69,14 @@ template <> struct Pair16<__nv_bfloat16> {
         return *reinterpret_cast<const uint32_t *>(&r);
     }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
     }
 };
 template <> struct Pair16<__half> {
@@ -81,9 +92,14 @@ template <> struct Pair16<__half> {
         return *reinterpret_cast<const uint32_t *>(&r);
     }
     static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+    static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
     }
 };
 template <typename E> struct MmaType { using T = E; };
@@ -100,198 +116,266 @@ template <typename H> __device__ __forceinline__ uint32_t code_pair(uint32_t wor
     return Pair16<H>::code(v, zero2);
 }
 
-// four consecutive activations of one token at column k, zeros beyond the row
-template <typename E> struct Quad {
-    uint32_t w[sizeof(E)];  // 4 elements: 2 or 4 words
-};
-template <typename E>
-__device__ __forceinline__ Quad<E> load_quad(const E *row, int64_t k, int64_t k_end, bool vec) {
-    Quad<E> q;
-    if (vec && k + 4 <= k_end) {
-        if constexpr (sizeof(E) == 2) {
-            const uint2 v = *reinterpret_cast<const uint2 *>(row + k);
-            q.w[0] = v.x, q.w[1] = v.y;
-        } else {
-            const uint4 v = *reinterpret_cast<const uint4 *>(row + k);
-            q.w[0] = v.x, q.w[1] = v.y, q.w[2] = v.z, q.w[3] = v.w;
-        }
-        return q;
-    }
-    E e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = k + i < k_end ? row[k + i] : E(0.f);
-    if constexpr (sizeof(E) == 2) {
-        const uint16_t *b = reinterpret_cast<const uint16_t *>(e);
-        q.w[0] = b[0] | (uint32_t)b[1] << 16, q.w[1] = b[2] | (uint32_t)b[3] << 16;
-    } else {
-        const uint32_t *b = reinterpret_cast<const uint32_t *>(e);
-        q.w[0] = b[0], q.w[1] = b[1], q.w[2] = b[2], q.w[3] = b[3];
-    }
-    return q;
+// x = b0 + b1 + b2 exactly: three bfloat16 terms, cut off rather than rounded, of eight significant bits
+// each (terms below the smallest bfloat16 are lost, far under the product's float32 rounding).
+// Infinities and NaN stay in the first term alone.  Two values at a time, packed.
+__device__ __forceinline__ void split3(uint32_t w0, uint32_t w1, uint32_t (&b)[3]) {
+    float x0 = __uint_as_float(w0) + 0.f, x1 = __uint_as_float(w1) + 0.f;  // makes a NaN quiet: its upper half is a NaN too
+    b[0] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+    x0 -= __uint_as_float(b[0] << 16);
+    x1 -= __uint_as_float(b[0] & 0xffff0000u);
+    x0 = x0 == x0 ? x0 : 0.f;
+    x1 = x1 == x1 ? x1 : 0.f;
+    b[1] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
+    x0 -= __uint_as_float(b[1] << 16);
+    x1 -= __uint_as_float(b[1] & 0xffff0000u);
+    b[2] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
 }
 
-// x = b[0] + b[1] + b[2] exactly: each bfloat16 term takes eight of the 24 significant bits (terms
-// below the smallest bfloat16 are lost, far under the product's float32 rounding).  Infinities and NaN
-// stay in the first term alone.
-__device__ __forceinline__ void split3(float x, __nv_bfloat16 (&b)[3]) {
-    b[0] = __float2bfloat16_rn(x);
-    float r = __bfloat162float(b[0]);
-    r = (isinf(r) || isnan(r)) ? 0.f : x - r;
-    if (isinf(__bfloat162float(b[0])) && !isinf(x)) b[0] = __float2bfloat16_rz(x), r = x - __bfloat162float(b[0]);
-    b[1] = __float2bfloat16_rn(r);
-    b[2] = __float2bfloat16_rn(r - __bfloat162float(b[1]));
+// SUB neighbouring values of type T as one register value (or vector of them)
+template <typename T, int SUB> struct Packed;
+template <> struct Packed<float, 1> { using V = float; static __device__ __forceinline__ float get(V v, int) { return v; } };
+template <> struct Packed<float, 2> { using V = float2; static __device__ __forceinline__ float get(V v, int i) { return i ? v.y : v.x; } };
+template <> struct Packed<float, 4> {
+    using V = float4;
+    static __device__ __forceinline__ float get(V v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+};
+template <> struct Packed<uint8_t, 1> { using V = uint8_t; static __device__ __forceinline__ float get(V v, int) { return (float)v; } };
+template <> struct Packed<uint8_t, 2> { using V = uint16_t; static __device__ __forceinline__ float get(V v, int i) { return (float)((v >> (8 * i)) & 0xff); } };
+template <> struct Packed<uint8_t, 4> { using V = uint32_t; static __device__ __forceinline__ float get(V v, int i) { return (float)((v >> (8 * i)) & 0xff); } };
+template <> struct Packed<int8_t, 1> { using V = int8_t; static __device__ __forceinline__ float get(V v, int) { return (float)v; } };
+template <> struct Packed<int8_t, 2> { using V = uint16_t; static __device__ __forceinline__ float get(V v, int i) { return (float)(int8_t)(v >> (8 * i)); } };
+template <> struct Packed<int8_t, 4> { using V = uint32_t; static __device__ __forceinline__ float get(V v, int i) { return (float)(int8_t)(v >> (8 * i)); } };
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <int SUB> struct SubScales {
-    float v[2][SUB];  // rows g and g + 8 of the tile
-};
-
-template <typename E, int NT, int SUB, bool ZEROS, bool MULT>
-__global__ void __launch_bounds__(kMvWarps * 32) k_matvec(Int4View w, const E *__restrict__ x, int64_t ldx, const E *__restrict__ bias,
-                                                          E *__restrict__ y, int64_t ldy, int tokens, int vec) {
+// A CTA takes up to kMvTiles tiles of 16 channels (all of their columns), or a cluster of `split` CTAs takes
+// one; `pass` tokens, at most eight, whose x lies in shared memory (float32: three bfloat16 planes) before
+// the first product.  The warps share the CTA's chunks evenly: a warp streams one contiguous run of codes, two
+// chunks requested ahead into registers, and leaves a partial sum for each of the at most two channel tiles
+// that it meets.
+template <typename E, int SUB, bool ZEROS, bool MULT>
+__global__ void __launch_bounds__(kMvWarps * 32, 2) k_matvec(Int4View w, const E *__restrict__ x, int64_t ldx, const E *__restrict__ bias,
+                                                             E *__restrict__ y, int64_t ldy, int tokens, int pass, int vec, int split) {
     using H = typename MmaType<E>::T;
-    constexpr bool F32 = sizeof(E) == 4;
-    constexpr int XW = sizeof(E);  // 32-bit words of a Quad
+    using S = std::conditional_t<MULT, uint8_t, float>;
+    using SP = Packed<S, SUB>;
+    using ZP = Packed<int8_t, SUB>;
+    constexpr bool F32 = sizeof(E) == 4, FINE = SUB == 4;
+    constexpr int P = F32 ? 3 : 1;
+    constexpr int NB = SUB == 4 && !MULT ? 1 : 2;  // chunks in registers
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float part[kMvWarps][2][128];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int64_t tile = blockIdx.x;
-    const int m0 = blockIdx.y * 8 * NT;
-    const int kt0 = (int)((int64_t)w.kt * warp / kMvWarps), kt1 = (int)((int64_t)w.kt * (warp + 1) / kMvWarps);
+    const uint32_t tiles = (uint32_t)div_up(w.n, kTileN);
+    const uint32_t cta = blockIdx.x, ctas = gridDim.x;
+    const uint32_t rank = split > 1 ? cta % split : 0;
+    // tiles [tile0, tile0 + n_tiles): the first `tiles % ctas` CTAs have one more
+    const uint32_t each = tiles / ctas, more = tiles % ctas;
+    const uint32_t tile0 = split > 1 ? cta / split : cta * each + min(cta, more), n_tiles = split > 1 ? 1 : each + (cta < more);
+    const uint32_t units = n_tiles * w.chunks, parts = kMvWarps * split;
+    auto unit_of = [&](uint32_t part) { return units * part / parts; };  // units <= 8 * 2^12, parts <= 64
+    const uint32_t u0 = unit_of(rank * kMvWarps + warp), u1 = unit_of(rank * kMvWarps + warp + 1);
+    const uint32_t row0 = u0 / w.chunks, turn = (row0 + 1) * w.chunks;  // first unit of the warp's second channel tile
+    const int m0 = blockIdx.y * pass;
+    tokens = min(tokens - m0, pass);
 
-    const uint4 *codes = w.codes + (tile * w.kt) * 32 + lane;
-    const int64_t entry0 = tile * w.entries;
-
-    uint4 cw[kMvDepth];
-    SubScales<SUB> cs[kMvDepth];
-    SubScales<SUB> cz[kMvDepth];
-    Quad<E> cx[kMvDepth][NT][4];
-
-    auto load_weights = [&](int slot, int kt) {
-        cw[slot] = __ldcs(codes + (int64_t)kt * 32);
-        const int64_t e = (entry0 + kt / w.per) * kTileN;
+    struct {
+        uint4 code[4];
+        typename SP::V scale[4][2];
+        typename ZP::V zero[4][2];
+    } buf[NB];
+    const uint4 *code_at = w.codes + ((uint64_t)tile0 * w.chunks + u0) * 128 + lane;
+    const int64_t entry0 = ((int64_t)tile0 * w.chunks + u0) * w.entries * kTileN + g;
+    const typename SP::V *scale_at = static_cast<const typename SP::V *>(w.scales) + entry0;
+    const typename ZP::V *zero_at = reinterpret_cast<const typename ZP::V *>(w.zeros) + (ZEROS ? entry0 : 0);
+    const int step = w.entries * kTileN;
+    const int off[4] = {0, w.entries / 4 * kTileN, w.entries / 2 * kTileN, w.entries * 3 / 4 * kTileN};  // of a tile's entry in a chunk
+    auto load = [&](int b) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const int64_t at = (e + g + 8 * r) * SUB;
+        for (int i = 0; i < 4; ++i) buf[b].code[i] = __ldcs(code_at + 32 * i);
 #pragma unroll
-            for (int i = 0; i < SUB; ++i) {
-                cs[slot].v[r][i] = MULT ? (float)static_cast<const uint8_t *>(w.scales)[at + i] : static_cast<const float *>(w.scales)[at + i];
-                if (ZEROS) cz[slot].v[r][i] = (float)w.zeros[at + i];
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int at = (SUB == 1 ? off[i] : kTileN * i) + 8 * r;
+                buf[b].scale[i][r] = scale_at[at];
+                if constexpr (ZEROS) buf[b].zero[i][r] = zero_at[at];
             }
-        }
+        code_at += 128;
+        scale_at += step;
+        if (ZEROS) zero_at += step;
     };
-    auto load_x = [&](int slot, int kt) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int m = m0 + 8 * j + g;
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                if (m < tokens)
-                    cx[slot][j][s] = load_quad(x + (int64_t)m * ldx, (int64_t)kt * kTileK + 16 * s + 4 * t, w.k, vec);
-                else
-#pragma unroll
-                    for (int i = 0; i < XW; ++i) cx[slot][j][s].w[i] = 0;
-            }
-        }
-    };
-
-    float total[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) total[j][i] = 0.f;
 
     // the weights are written by no kernel that lets its successor start early (aimet_b200_int4_pack
     // does not), so they may be requested before the wait for the predecessor; x may not
     pdl_launch_dependents();
 #pragma unroll
-    for (int d = 0; d < kMvDepth; ++d)
-        if (kt0 + d < kt1) load_weights(d, kt0 + d);
+    for (int b = 0; b < NB; ++b)
+        if (u0 + b < u1) load(b);
     pdl_wait();
-#pragma unroll
-    for (int d = 0; d < kMvDepth; ++d)
-        if (kt0 + d < kt1) load_x(d, kt0 + d);
 
-    for (int base = kt0; base < kt1; base += kMvDepth) {
+    const uint32_t pitch = w.chunks * (kChunkK * 2) + 64;  // 64 modulo 128: the reads of eight lanes meet no bank twice
+    // 16-byte pieces of x: a thread takes two columns of four tokens at once
+    constexpr int V = 16 / sizeof(E), MA = 4, CA = 2;
+    const int per_row = w.chunks * (kChunkK / V);
+    const uint32_t plane = pass * pitch;
+    auto put = [&](const Vec16<E> &v, int m, int c) {
+        uint8_t *dst = smem + m * pitch + 2 * V * c;
+        if constexpr (F32) {
+            uint32_t lo[3], hi[3];
+            split3(__float_as_uint(v.v[0]), __float_as_uint(v.v[1]), lo);
+            split3(__float_as_uint(v.v[2]), __float_as_uint(v.v[3]), hi);
 #pragma unroll
-        for (int d = 0; d < kMvDepth; ++d) {
-            const int kt = base + d;
-            if (kt >= kt1) break;
-            const uint32_t word[4] = {cw[d].x, cw[d].y, cw[d].z, cw[d].w};
-            float acc[NT][4];
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const int sub = s * SUB / 4;
-                uint32_t z0, z1;
-                if (ZEROS) {
-                    z0 = zero_pair<H>(cz[d].v[0][sub]);
-                    z1 = zero_pair<H>(cz[d].v[1][sub]);
-                } else {
-                    z0 = z1 = zero_pair<H>(w.zero);
-                }
-                const int p = 2 * (s & 1), q = 2 * (s >> 1);
-                const uint32_t a[4] = {code_pair<H>(word[q], p, z0), code_pair<H>(word[q + 1], p, z1),
-                                       code_pair<H>(word[q], p + 1, z0), code_pair<H>(word[q + 1], p + 1, z1)};
-                if (s % (4 / SUB) == 0) {
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[j][i] = 0.f;
-                }
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const Quad<E> &q4 = cx[d][j][s];
-                    if constexpr (F32) {
-                        __nv_bfloat16 b[4][3];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) split3(__uint_as_float(q4.w[i]), b[i]);
-#pragma unroll
-                        for (int e = 0; e < 3; ++e) {
-                            const __nv_bfloat162 lo = __halves2bfloat162(b[0][e], b[1][e]), hi = __halves2bfloat162(b[2][e], b[3][e]);
-                            Pair16<H>::mma(acc[j], a, *reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-                        }
-                    } else {
-                        Pair16<H>::mma(acc[j], a, q4.w[0], q4.w[1]);
-                    }
-                }
-                if (s % (4 / SUB) == 4 / SUB - 1) {
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) total[j][i] = fmaf(acc[j][i], cs[d].v[i >> 1][sub] * (1.f / Pair16<H>::kUnit), total[j][i]);
-                }
-            }
-            if (kt + kMvDepth < kt1) {
-                load_weights(d, kt + kMvDepth);
-                load_x(d, kt + kMvDepth);
-            }
+            for (int e = 0; e < 3; ++e) *reinterpret_cast<uint2 *>(dst + e * plane) = make_uint2(lo[e], hi[e]);
+        } else {
+            *reinterpret_cast<Vec16<E> *>(dst) = v;
         }
-    }
-
-    // the warps' sums, added in a fixed order
-    __shared__ float part[kMvWarps][NT * 128];
+    };
+    if (vec) {  // whole pieces, 16-byte aligned
+        const int have = (int)(w.k / V);
+        for (int m = 0; m < tokens; m += MA)
+            for (int c = threadIdx.x; c < per_row; c += CA * kMvWarps * 32) {
+                uint4 v[MA][CA];
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+                for (int i = 0; i < MA; ++i)
+#pragma unroll
+                    for (int j = 0; j < CA; ++j) {
+                        const int cc = c + j * kMvWarps * 32;
+                        v[i][j] = make_uint4(0, 0, 0, 0);
+                        if (m + i < tokens && cc < have) v[i][j] = *reinterpret_cast<const uint4 *>(x + (int64_t)(m0 + m + i) * ldx + cc * V);
+                    }
+#pragma unroll
+                for (int i = 0; i < MA; ++i)
+#pragma unroll
+                    for (int j = 0; j < CA; ++j) {
+                        const int cc = c + j * kMvWarps * 32;
+                        if (m + i < tokens && cc < per_row) put(*reinterpret_cast<const Vec16<E> *>(&v[i][j]), m + i, cc);
+                    }
+            }
+    } else {
+        for (int m = 0; m < tokens; ++m)
+            for (int c = threadIdx.x; c < per_row; c += kMvWarps * 32) {
+                Vec16<E> v;
+#pragma unroll
+                for (int j = 0; j < V; ++j) v.v[j] = c * V + j < w.k ? x[(int64_t)(m0 + m) * ldx + c * V + j] : E(0.f);
+                put(v, m, c);
+            }
+    }
+    __syncthreads();
+
+    // Columns of the product are tokens: a lane whose token does not exist multiplies some other token's x
+    // into a column that nobody stores.
+    const uint8_t *xs = smem + (size_t)min(g, tokens - 1) * pitch + (FINE ? 8 : 16) * t;
+    const uint32_t one_zero = zero_pair<H>(w.zero);
+    float total[4] = {0.f, 0.f, 0.f, 0.f};
+    auto leave = [&](int segment) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int m = 8 * j + 2 * t + (i & 1), row = g + 8 * (i >> 1);
-            part[warp][m * 16 + row] = total[j][i];
+            part[warp][segment][(2 * t + (i & 1)) * 16 + g + 8 * (i >> 1)] = total[i];
+            total[i] = 0.f;
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < NT * 128; i += kMvWarps * 32) {
-        const int m = m0 + (i >> 4);
-        const int64_t n = tile * kTileN + (i & 15);
-        if (m >= tokens || n >= w.n) continue;
-        float v = 0.f;
+    };
+    for (uint32_t base = u0; base < u1; base += NB) {
 #pragma unroll
-        for (int q = 0; q < kMvWarps; ++q) v += part[q][i];
-        if (MULT) v *= w.row_scale[n];
-        if (bias) v += to_f32(bias[n]);
-        y[(int64_t)m * ldy + n] = Cvt<float, E>::store(v);
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t u = base + b;
+            if (u >= u1) break;
+            if (u == turn) leave(0);
+            const uint8_t *xc = xs + (u - (u >= turn ? turn : turn - w.chunks)) * (kChunkK * 2);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint4 v[2][P];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < P; ++e) {
+                        const uint8_t *p = xc + e * plane + i * 128 + 64 * h;
+                        if constexpr (FINE) {
+                            const uint2 lo = *reinterpret_cast<const uint2 *>(p), hi = *reinterpret_cast<const uint2 *>(p + 32);
+                            v[h][e] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                        } else {
+                            v[h][e] = *reinterpret_cast<const uint4 *>(p);
+                        }
+                    }
+                const uint4 w4 = buf[b].code[i];
+                const uint32_t word[4] = {w4.x, w4.y, w4.z, w4.w};
+                float acc[4];
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    const int sub = s * SUB / 4, p = 2 * (s & 1), q = 2 * (s >> 1);
+                    const uint32_t z0 = ZEROS ? zero_pair<H>(ZP::get(buf[b].zero[i][0], sub)) : one_zero;
+                    const uint32_t z1 = ZEROS ? zero_pair<H>(ZP::get(buf[b].zero[i][1], sub)) : one_zero;
+                    const uint32_t a[4] = {code_pair<H>(word[q], p, z0), code_pair<H>(word[q + 1], p, z1),
+                                           code_pair<H>(word[q], p + 1, z0), code_pair<H>(word[q + 1], p + 1, z1)};
+#pragma unroll
+                    for (int e = 0; e < P; ++e) {
+                        const uint32_t b0 = (s & 1) ? v[s >> 1][e].z : v[s >> 1][e].x, b1 = (s & 1) ? v[s >> 1][e].w : v[s >> 1][e].y;
+                        if (s % (4 / SUB) == 0 && e == 0)
+                            Pair16<H>::mma_first(acc, a, b0, b1);
+                        else
+                            Pair16<H>::mma(acc, a, b0, b1);
+                    }
+                    if (s % (4 / SUB) == 4 / SUB - 1) {
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const float f = SP::get(buf[b].scale[i][r], sub);
+                            total[2 * r] = fmaf(acc[2 * r], f, total[2 * r]);
+                            total[2 * r + 1] = fmaf(acc[2 * r + 1], f, total[2 * r + 1]);
+                        }
+                    }
+                }
+            }
+            if (u + NB < u1) load(b);
+        }
     }
+    leave(u1 > turn ? 1 : 0);
+
+    // the warps' sums of every channel tile, added in a fixed order
+    if (split > 1)
+        cluster_barrier();
+    else
+        __syncthreads();
+    if (rank == 0) {
+        for (uint32_t i = threadIdx.x; i < n_tiles * 128; i += kMvWarps * 32) {
+            const uint32_t row = i / 128, at = i % 128;
+            const int m = (int)(at >> 4);
+            const int64_t n = (int64_t)(tile0 + row) * kTileN + (at & 15);
+            if (m >= tokens || n >= w.n) continue;
+            float v = 0.f;
+            if (split > 1) {
+                const uint32_t here = (uint32_t)__cvta_generic_to_shared(&part[0][0][at]);
+                for (int c = 0; c < split; ++c) {
+                    uint32_t there;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
+#pragma unroll
+                    for (int q = 0; q < kMvWarps; ++q) {
+                        float f;
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there + q * (2 * 128 * 4)) : "memory");
+                        v += f;
+                    }
+                }
+            } else {
+                const uint32_t lo = row * w.chunks, hi = lo + w.chunks;
+#pragma unroll
+                for (int q = 0; q < kMvWarps; ++q) {
+                    const uint32_t a = unit_of(q), b = unit_of(q + 1);
+                    if (a < hi && b > lo && a < b) v += part[q][a < lo ? 1 : 0][at];
+                }
+            }
+            v *= w.row_scale[n] * (1.f / Pair16<H>::kUnit);
+            if (bias) v += to_f32(bias[n]);
+            y[(int64_t)(m0 + m) * ldy + n] = Cvt<float, E>::store(v);
+        }
+    }
+    if (split > 1) cluster_barrier();  // nobody of the cluster leaves while its sums are being read
 }
 
 // codes [n][k] (one signed byte each, qmin .. qmin + 15) -> the tiled 4-bit layout; what lies outside
 // the matrix gets code 0, which meets zeros of x.
-__global__ void k_int4_pack(const int8_t *__restrict__ codes, int64_t n, int64_t k, int kt, int qmin, uint4 *__restrict__ out, int64_t total) {
+__global__ void k_int4_pack(const int8_t *__restrict__ codes, int64_t n, int64_t k, int kt, int qmin, int fine, uint4 *__restrict__ out, int64_t total) {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= total) return;
     const int lane = (int)(i & 31), g = lane >> 2, t = lane & 3;
@@ -305,7 +389,7 @@ __global__ void k_int4_pack(const int8_t *__restrict__ codes, int64_t n, int64_t
         for (int p = 0; p < 4; ++p) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int64_t c = col * kTileK + 16 * (2 * (q >> 1) + (p >> 1)) + 4 * t + 2 * (p & 1) + h;
+                const int64_t c = col * kTileK + 32 * (q >> 1) + (fine ? 16 * (p >> 1) + 4 * t : 4 * (p >> 1) + 8 * t) + 2 * (p & 1) + h;
                 const int u = row < n && c < k ? (int)codes[row * k + c] - qmin : 0;
                 v |= (uint32_t)(u & 15) << (4 * p + 16 * h);
             }
@@ -315,16 +399,18 @@ __global__ void k_int4_pack(const int8_t *__restrict__ codes, int64_t n, int64_t
     out[i] = make_uint4(word[0], word[1], word[2], word[3]);
 }
 
+bool storable(int block) { return block == 16 || block == 32 || block == 64 || block == 128 || block == 256; }
+
 int check_weight(const ab_int4_weight *w, Int4View *v) {
     if (!w) return fail(AB_ERR_INVALID, "weight is NULL");
-    if (w->n < 1 || w->k < 1 || w->n > (1ll << 30) || w->k > (1ll << 30))
+    if (w->n < 1 || w->k < 1 || w->n > (1ll << 30) || w->k > kMaxK)
         return fail(AB_ERR_INVALID, "weight of %lld x %lld", (long long)w->n, (long long)w->k);
-    if (w->block != 16 && w->block != 32 && (w->block < 64 || w->block % 64))
-        return fail(AB_ERR_UNSUPPORTED, "storage block %d: 16, 32 or a multiple of 64", w->block);
+    if (!storable(w->block)) return fail(AB_ERR_UNSUPPORTED, "storage block %d: 16, 32, 64, 128 or 256", w->block);
     if (!w->codes || !w->scales) return fail(AB_ERR_INVALID, "codes or scales is NULL");
-    if (!aligned16(w->codes)) return fail(AB_ERR_INVALID, "codes must be 16-byte aligned");
+    if (!aligned16(w->codes) || !aligned16(w->scales) || !aligned16(w->zeros))
+        return fail(AB_ERR_INVALID, "codes, scales and zeros must be 16-byte aligned");
     if (w->scale_kind != 0 && w->scale_kind != 1) return fail(AB_ERR_INVALID, "scale_kind %d", w->scale_kind);
-    if (w->scale_kind == 1 && !w->row_scale) return fail(AB_ERR_INVALID, "scale_kind 1 needs row_scale");
+    if (!w->row_scale) return fail(AB_ERR_INVALID, "row_scale is NULL");
     if (!w->zeros && (w->zero < -112 || w->zero > 112)) return fail(AB_ERR_INVALID, "zero point %d outside [-112, 112]", w->zero);
     v->codes = static_cast<const uint4 *>(w->codes);
     v->scales = w->scales;
@@ -332,9 +418,8 @@ int check_weight(const ab_int4_weight *w, Int4View *v) {
     v->row_scale = static_cast<const float *>(w->row_scale);
     v->n = w->n;
     v->k = w->k;
-    v->kt = (int)div_up(w->k, kTileK);
-    v->per = w->block <= kTileK ? 1 : w->block / kTileK;
-    v->entries = (int)div_up(v->kt, v->per);
+    v->chunks = (int)div_up(w->k, kChunkK);
+    v->entries = w->block <= kTileK ? 4 : kChunkK / w->block;
     v->zero = (float)w->zero;
     return AB_OK;
 }
@@ -348,28 +433,60 @@ struct MatvecCall {
     cudaStream_t stream;
 };
 
-template <typename E, int NT, int SUB, bool ZEROS, bool MULT> int launch_matvec(const MatvecCall &c) {
-    constexpr int kMost = 65535 * 8 * NT;  // tokens of one launch: the grid's second dim
-    for (int64_t m = 0; m < c.tokens; m += kMost) {
-        const int tokens = (int)std::min<int64_t>(kMost, c.tokens - m);
-        const dim3 grid((unsigned)div_up(c.w.n, kTileN), (unsigned)div_up(tokens, 8 * NT));
-        AB_CUDA_OK(launch_pdl(k_matvec<E, NT, SUB, ZEROS, MULT>, grid, dim3(kMvWarps * 32), 0, c.stream, c.w,
-                              static_cast<const E *>(c.x) + m * c.ldx, c.ldx, static_cast<const E *>(c.bias),
-                              static_cast<E *>(c.y) + m * c.ldy, c.ldy, tokens, c.vec));
+constexpr size_t kMvSmem = 218 * 1024, kMvSmemHalf = 104 * 1024;  // one CTA on an SM, two (beside 8 KB of sums each)
+
+template <typename E, int SUB, bool ZEROS, bool MULT> int launch_matvec(const MatvecCall &c) {
+    const auto kernel = k_matvec<E, SUB, ZEROS, MULT>;
+    const size_t row = (size_t)(sizeof(E) == 4 ? 3 : 1) * (c.w.chunks * (kChunkK * 2) + 64);  // x of a token
+    if (row > kMvSmem)
+        return fail(AB_ERR_UNSUPPORTED, "%lld input channels: x of one token does not fit shared memory", (long long)c.w.k);
+    const int rc = opt_in_smem<k_matvec<E, SUB, ZEROS, MULT>>(kMvSmem);
+    if (rc != AB_OK) return rc;
+    const int64_t tiles = div_up(c.w.n, kTileN);
+    const int sms = sm_count();
+    // Tokens that are multiplied in one pass over the weights (a second pass finds them in L2): eight, or what
+    // leaves room for a second CTA on the SM.
+    int pass = (int)std::min<size_t>(8, std::max<size_t>(1, kMvSmemHalf / row));
+    pass = (int)div_up(c.tokens, div_up(c.tokens, pass));
+
+    constexpr int kMost = 65535;  // passes of one launch: the grid's second dim
+    for (int64_t m = 0; m < c.tokens; m += (int64_t)kMost * pass) {
+        const int tokens = (int)std::min<int64_t>((int64_t)kMost * pass, c.tokens - m);
+        const int64_t passes = div_up(tokens, pass);
+        // Two CTAs per SM and no more than kMvTiles channel tiles for one.  Few channel tiles: a cluster of
+        // CTAs per tile, while that leaves a chunk for every warp.
+        const int64_t slots = div_up(sms * 2, passes);
+        int split = 1;
+        while (split < 8 && tiles * split * 2 <= slots && c.w.chunks >= split * 2 * kMvWarps) split *= 2;
+        const int64_t ctas = split > 1 ? tiles * split : std::min(tiles, std::max(slots, div_up(tiles, kMvTiles)));
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)ctas, (unsigned)passes);
+        cfg.blockDim = dim3(kMvWarps * 32);
+        cfg.dynamicSmemBytes = row * pass;
+        cfg.stream = c.stream;
+        cudaLaunchAttribute attr[2];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = split;
+        attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = split > 1 ? 2 : 1;
+        AB_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, c.w, static_cast<const E *>(c.x) + m * c.ldx, c.ldx, static_cast<const E *>(c.bias),
+                                      static_cast<E *>(c.y) + m * c.ldy, c.ldy, tokens, pass, c.vec, split));
         AB_LAUNCH_OK();
     }
     return AB_OK;
 }
-template <typename E, int NT, int SUB> int dispatch_scales(const MatvecCall &c, bool mult) {
-    if (mult) return c.w.zeros ? launch_matvec<E, NT, SUB, true, true>(c) : launch_matvec<E, NT, SUB, false, true>(c);
-    return c.w.zeros ? launch_matvec<E, NT, SUB, true, false>(c) : launch_matvec<E, NT, SUB, false, false>(c);
+template <typename E, int SUB> int dispatch_scales(const MatvecCall &c, bool mult) {
+    if (mult) return c.w.zeros ? launch_matvec<E, SUB, true, true>(c) : launch_matvec<E, SUB, false, true>(c);
+    return c.w.zeros ? launch_matvec<E, SUB, true, false>(c) : launch_matvec<E, SUB, false, false>(c);
 }
-template <typename E, int NT> int dispatch_block(const MatvecCall &c, int block, bool mult) {
-    if (block == 16) return dispatch_scales<E, NT, 4>(c, mult);
-    if (block == 32) return dispatch_scales<E, NT, 2>(c, mult);
-    return dispatch_scales<E, NT, 1>(c, mult);
+template <typename E> int dispatch_matvec(const MatvecCall &c, int block, bool mult) {
+    if (block == 16) return dispatch_scales<E, 4>(c, mult);
+    if (block == 32) return dispatch_scales<E, 2>(c, mult);
+    return dispatch_scales<E, 1>(c, mult);
 }
-template <typename E> int dispatch_tokens(const MatvecCall &c, int block, bool mult) { return dispatch_block<E, 1>(c, block, mult); }
 
 }  // namespace
 }  // namespace ab
@@ -377,11 +494,12 @@ template <typename E> int dispatch_tokens(const MatvecCall &c, int block, bool m
 using namespace ab;
 
 extern "C" int64_t aimet_b200_int4_codes_bytes(int64_t n, int64_t k) {
-    if (n < 1 || k < 1 || n > (1ll << 30) || k > (1ll << 30)) return fail(AB_ERR_INVALID, "weight of %lld x %lld", (long long)n, (long long)k);
-    return div_up(n, kTileN) * div_up(k, kTileK) * 512;
+    if (n < 1 || k < 1 || n > (1ll << 30) || k > kMaxK) return fail(AB_ERR_INVALID, "weight of %lld x %lld", (long long)n, (long long)k);
+    return div_up(n, kTileN) * div_up(k, kChunkK) * 2048;
 }
 
-extern "C" int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int qmin, void *out, void *stream) {
+extern "C" int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int qmin, int block, void *out, void *stream) {
+    if (!storable(block)) return fail(AB_ERR_UNSUPPORTED, "storage block %d: 16, 32, 64, 128 or 256", block);
     const int64_t bytes = aimet_b200_int4_codes_bytes(n, k);
     if (bytes < 0) return (int)bytes;
     if (!codes || !out) return fail(AB_ERR_INVALID, "codes or out is NULL");
@@ -391,7 +509,7 @@ extern "C" int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int
     const int64_t blocks = div_up(total, 256);
     if (blocks > 0x7fffffff) return fail(AB_ERR_UNSUPPORTED, "weight of %lld x %lld is too large", (long long)n, (long long)k);
     k_int4_pack<<<(unsigned)blocks, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const int8_t *>(codes), n, k, (int)div_up(k, kTileK), qmin, static_cast<uint4 *>(out), total);
+        static_cast<const int8_t *>(codes), n, k, (int)div_up(k, kChunkK) * (kChunkK / kTileK), qmin, block == 16, static_cast<uint4 *>(out), total);
     AB_LAUNCH_OK();
     return AB_OK;
 }
@@ -414,12 +532,12 @@ extern "C" int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *
     c.ldx = ldx;
     c.ldy = ldy;
     c.tokens = (int)tokens;
-    c.vec = reinterpret_cast<uintptr_t>(x) % (4 * size) == 0 && (ldx % 4 == 0 || tokens == 1);
+    c.vec = aligned16(x) && weight->k * size % 16 == 0 && (ldx * size % 16 == 0 || tokens == 1);
     c.stream = static_cast<cudaStream_t>(stream);
     const bool mult = weight->scale_kind == 1;
     switch (io_dtype) {
-        case AB_F32: return dispatch_tokens<float>(c, weight->block, mult);
-        case AB_F16: return dispatch_tokens<__half>(c, weight->block, mult);
-        default: return dispatch_tokens<__nv_bfloat16>(c, weight->block, mult);
+        case AB_F32: return dispatch_matvec<float>(c, weight->block, mult);
+        case AB_F16: return dispatch_matvec<__half>(c, weight->block, mult);
+        default: return dispatch_matvec<__nv_bfloat16>(c, weight->block, mult);
     }
 }

@@ -20,32 +20,34 @@ from ._lib import check, lib
 
 __all__ = ["PackedInt4Weight", "linear_int4"]
 
-_TILE_N, _TILE_K = 16, 64
+_TILE_N, _TILE_K, _CHUNK_K = 16, 64, 256
 _MAX_ZERO = 112  # 16-bit floats subtract zero points up to here exactly
 
 
 def _storage_block(block: int, in_features: int) -> int:
-    """Input channels per scale as the kernels store them: 16, 32 or a multiple of 64 that divides
-    ``block``; a scale for the whole row counts as the next multiple of 64."""
+    """Input channels per scale as the kernels store them: the largest of 16, 32, 64, 128 and 256 that
+    divides ``block`` (a scale for the whole row is stored for every 256)."""
     if block == in_features:
-        return -(-in_features // _TILE_K) * _TILE_K
-    for b in (64, 32, 16):
+        return _CHUNK_K
+    for b in (256, 128, 64, 32, 16):
         if block % b == 0:
-            return block if b == 64 else b
+            return b
     raise NotImplementedError(f"blocks of {block} input channels: a multiple of 16, or the whole row, is supported")
 
 
 def _tiled(param: torch.Tensor, block: int, storage: int, in_features: int) -> torch.Tensor:
-    """[out, blocks] -> the kernels' order [ceil(out / 16)][entries][16][sub] (zeros behind the matrix)."""
+    """[out, blocks] -> the kernels' order [ceil(out / 16)][chunk of 256 columns][entry][16][sub] (zeros
+    behind the matrix)."""
     n = param.shape[0]
-    sub = max(1, _TILE_K // storage)
-    tiles = -(-in_features // _TILE_K)
-    entries = -(-tiles // max(1, storage // _TILE_K))
-    if block != in_features and storage != block:
+    chunks, sub = -(-in_features // _CHUNK_K), max(1, _TILE_K // storage)
+    entries = _CHUNK_K // max(_TILE_K, storage)
+    if block == in_features:
+        param = param.expand(n, chunks)
+    elif storage != block:
         param = param.repeat_interleave(block // storage, 1)
-    out = param.new_zeros(-(-n // _TILE_N) * _TILE_N, entries * sub)
+    out = param.new_zeros(-(-n // _TILE_N) * _TILE_N, chunks * entries * sub)
     out[:n, : param.shape[1]] = param
-    return out.view(-1, _TILE_N, entries, sub).permute(0, 2, 1, 3).contiguous()
+    return out.view(-1, _TILE_N, chunks, entries, sub).permute(0, 2, 3, 1, 4).contiguous()
 
 
 class PackedInt4Weight:
@@ -55,13 +57,13 @@ class PackedInt4Weight:
     ``w[n, k] = (code[n, k] + offset[n, b]) * scale[n, b]`` with ``b`` the block of column ``k``.
     """
 
-    def __init__(self, out_features, in_features, block_size, qmin, codes, scales, zeros, row_scale, zero):
+    def __init__(self, out_features, in_features, block_size, qmin, codes, scales, multiples, zeros, row_scale, zero):
         self.out_features, self.in_features = out_features, in_features
         self.block_size, self.qmin = block_size, qmin
         self._buffers = (codes, scales, zeros, row_scale)  # what the descriptor below points at
         storage = _storage_block(block_size, in_features)
-        self._desc = _lib.Int4Weight(out_features, in_features, storage, int(row_scale is not None), zero, 0,
-                                     codes.data_ptr(), scales.data_ptr(), _lib.ptr(zeros), _lib.ptr(row_scale))
+        self._desc = _lib.Int4Weight(out_features, in_features, storage, int(multiples), zero, 0,
+                                     codes.data_ptr(), scales.data_ptr(), _lib.ptr(zeros), row_scale.data_ptr())
         self.device = codes.device
 
     @property
@@ -107,9 +109,14 @@ class PackedInt4Weight:
             whole = codes.to(torch.int32)
             if bool(((whole != codes) | (whole < qmin) | (whole > qmin + 15)).any()):
                 raise RuntimeError(f"codes must be whole numbers in [{qmin}, {qmin + 15}]")
-            row_scale = None
             if int_scale is None:
-                scales = _tiled(scale.detach().to(torch.float32), block, storage, k)
+                # a power of two per channel is split off, so that what many tokens multiply in 16 bits has a
+                # channel's largest scale near 1 whatever the size of the weights
+                scale = scale.detach().to(torch.float32)
+                top = scale.abs().amax(1)
+                top = torch.where(torch.isfinite(top) & (top > 0), top, torch.ones_like(top))
+                row_scale = torch.ldexp(torch.ones_like(top), torch.frexp(top).exponent.clamp(-125, 127))
+                scales = _tiled(scale / row_scale[:, None], block, storage, k)
             else:
                 if bool(((int_scale != int_scale.to(torch.uint8)) | (int_scale < 0) | (int_scale > 255)).any()):
                     raise RuntimeError("int_scale must hold whole numbers in [0, 255]")
@@ -129,8 +136,9 @@ class PackedInt4Weight:
             codes8 = whole.to(torch.int8).contiguous()
             packed = torch.empty(lib.aimet_b200_int4_codes_bytes(n, k), dtype=torch.uint8, device=codes.device)
             with _lib.on_device(codes.device):
-                check(lib.aimet_b200_int4_pack(codes8.data_ptr(), n, k, qmin, packed.data_ptr(), _lib.stream_ptr(codes.device)))
-        return cls(n, k, block, qmin, packed, scales, zeros, row_scale, zero)
+                check(lib.aimet_b200_int4_pack(codes8.data_ptr(), n, k, qmin, storage, packed.data_ptr(),
+                                               _lib.stream_ptr(codes.device)))
+        return cls(n, k, block, qmin, packed, scales, int_scale is not None, zeros, row_scale, zero)
 
     @classmethod
     def from_encoding(cls, weight: torch.Tensor, encoding) -> "PackedInt4Weight":

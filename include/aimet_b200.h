@@ -393,17 +393,19 @@ int aimet_b200_seqmse_wait_selftest(int32_t *status, int64_t limit_us, void *str
  *   w[i][j] = (code[i][j] + offset[i][g]) * scale[i][g],  code in [qmin, qmin + 15]
  * codes: aimet_b200_int4_codes_bytes() bytes written by aimet_b200_int4_pack (u = code - qmin).
  * scales, zeros: one entry per channel and block, stored as
- *   [ceil(n / 16)][ceil(tiles / per)][16][sub],  tiles = ceil(k / 64), per = max(1, block / 64),
- *   sub = max(1, 64 / block): entry [i / 16][..][i % 16][..] belongs to channel i, zeros in what
- *   lies behind the matrix.
- * scale_kind 0: scales are float32.  scale_kind 1: scales are uint8 factors of row_scale[channel]
- * (float32, one per channel): the blockwise grid of GroupedBlockQuantizeDequantize.
+ *   [ceil(n / 16)][ceil(k / 256)][entries][16][sub],  entries = 256 / max(64, block),
+ *   sub = max(1, 64 / block): channel i, column j finds its own at
+ *   [i / 16][j / 256][j % 256 / max(64, block)][i % 16][j % 64 / block]; any finite value behind the matrix.
+ * The scale of a block is its entry times row_scale[channel] (float32, one per channel).  scale_kind 0:
+ * entries are float32, at most 1 in magnitude, row_scale a power of two (so that the product is the
+ * scale exactly).  scale_kind 1: entries are uint8 factors: the blockwise grid of
+ * GroupedBlockQuantizeDequantize.
  * zeros: int8, z = -(qmin + offset) per channel and block, |z| <= 112 (what 16-bit floats subtract
  * exactly); NULL: `zero` for all.
  * ------------------------------------------------------------------------- */
 typedef struct ab_int4_weight {
     int64_t n, k;       /* output channels, input channels */
-    int32_t block;      /* input channels per scale: 16, 32 or a multiple of 64 */
+    int32_t block;      /* input channels per stored scale: 16, 32, 64, 128 or 256 */
     int32_t scale_kind; /* 0 float32, 1 uint8 factors of row_scale */
     int32_t zero;       /* zero point where zeros is NULL */
     int32_t reserved;
@@ -411,8 +413,9 @@ typedef struct ab_int4_weight {
 } ab_int4_weight;
 
 int64_t aimet_b200_int4_codes_bytes(int64_t n, int64_t k);
-/* codes: int8 [n][k], each in [qmin, qmin + 15] (the four low bits of code - qmin are kept) */
-int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int qmin, void *out, void *stream);
+/* codes: int8 [n][k], each in [qmin, qmin + 15] (the four low bits of code - qmin are kept); block as in
+ * ab_int4_weight (blocks of 16 have a column order of their own) */
+int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int qmin, int block, void *out, void *stream);
 /* y[m][i] = sum_j x[m][j] * w[i][j] + bias[i] for `tokens` rows; x rows are ldx elements apart, y rows
  * ldy; bias (io_dtype, n elements) may be NULL.  Float32 accumulation, one rounding to io_dtype. */
 int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *x, int64_t ldx, const void *bias, void *y,

@@ -10,39 +10,40 @@ import torch
 def test_storage_blocks_and_tiled_scales():
     from aimet_b200 import int4
 
-    assert [int4._storage_block(b, 1024) for b in (16, 32, 48, 64, 96, 128, 192, 1024)] == [16, 32, 16, 64, 32, 128, 192, 1024]
-    assert int4._storage_block(77, 77) == 128 and int4._storage_block(1, 1) == 64
+    assert [int4._storage_block(b, 2048) for b in (16, 32, 48, 64, 96, 128, 192, 256, 512, 2048)] == [16, 32, 16, 64, 32, 128, 64, 256, 256, 256]
+    assert int4._storage_block(77, 77) == 256 and int4._storage_block(1, 1) == 256
     for bad in (8, 20, 40 + 2):
         with pytest.raises(NotImplementedError, match="multiple of 16"):
             int4._storage_block(bad, bad * 4)
-    # channel n, column c finds its scale at [n // 16][c // 64 // per][n % 16][c % 64 // storage]
-    for n, k, block in ((5, 96, 32), (20, 64, 16), (17, 384, 128), (16, 96, 48), (3, 77, 77), (33, 640, 320)):
+    # channel i, column j finds its scale at [i // 16][j // 256][j % 256 // max(64, block)][i % 16][j % 64 // block]
+    for n, k, block in ((5, 96, 32), (20, 64, 16), (17, 384, 128), (16, 96, 48), (3, 77, 77), (33, 640, 320), (2, 1024, 512), (3, 600, 600)):
         blocks = k // block
         param = torch.arange(n * blocks, dtype=torch.float32).view(n, blocks) + 1
         storage = int4._storage_block(block, k)
         tiled = int4._tiled(param, block, storage, k)
-        per = max(1, storage // 64)
-        assert tiled.is_contiguous() and tiled.shape[0] == -(-n // 16) and tiled.shape[2] == 16
+        assert tiled.is_contiguous() and tiled.shape[3] == 16
         for row in (0, n - 1):
-            for c in (0, 15, 16, 63, k // 2, k - 1):
-                if c < k:
-                    assert tiled[row // 16, c // 64 // per, row % 16, c % 64 // storage if storage < 64 else 0] == param[row, c // block]
+            for j in (0, 15, 16, 63, k // 2, k - 1):
+                if j < k:
+                    at = (row // 16, j // 256, j % 256 // max(64, storage), row % 16, j % 64 // storage)
+                    assert tiled[at] == param[row, j // block]
         if n % 16:
-            assert bool((tiled[-1, :, n % 16:] == 0).all())
+            assert bool((tiled[-1, :, :, n % 16:] == 0).all())
 
 
 def test_entry_points_refuse_before_touching_the_device():
     from aimet_b200 import _lib
 
     lib, one = _lib.lib, 1 << 20  # any aligned non-NULL value: the calls below return before a pointer is used
-    assert lib.aimet_b200_int4_codes_bytes(16, 64) == 512 and lib.aimet_b200_int4_codes_bytes(17, 65) == 4 * 512
+    assert lib.aimet_b200_int4_codes_bytes(16, 256) == 2048 and lib.aimet_b200_int4_codes_bytes(17, 257) == 4 * 2048
     assert lib.aimet_b200_int4_codes_bytes(0, 64) == _lib.AB_ERR_INVALID
-    assert lib.aimet_b200_int4_pack(one, 16, 64, -200, one, None) == _lib.AB_ERR_INVALID and "signed bytes" in _lib.last_error()
-    assert lib.aimet_b200_int4_pack(one, 16, 64, 0, one + 4, None) == _lib.AB_ERR_INVALID and "aligned" in _lib.last_error()
-    assert lib.aimet_b200_int4_pack(None, 16, 64, 0, one, None) == _lib.AB_ERR_INVALID
+    assert lib.aimet_b200_int4_pack(one, 16, 64, -200, 64, one, None) == _lib.AB_ERR_INVALID and "signed bytes" in _lib.last_error()
+    assert lib.aimet_b200_int4_pack(one, 16, 64, 0, 64, one + 4, None) == _lib.AB_ERR_INVALID and "aligned" in _lib.last_error()
+    assert lib.aimet_b200_int4_pack(one, 16, 64, 0, 48, one, None) == _lib.AB_ERR_UNSUPPORTED
+    assert lib.aimet_b200_int4_pack(None, 16, 64, 0, 64, one, None) == _lib.AB_ERR_INVALID
 
     def weight(**kw):
-        w = _lib.Int4Weight(32, 128, 64, 0, 8, 0, one, one, None, None)
+        w = _lib.Int4Weight(32, 128, 64, 0, 8, 0, one, one, None, one)
         for name, v in kw.items():
             setattr(w, name, v)
         return w
@@ -51,7 +52,7 @@ def test_entry_points_refuse_before_touching_the_device():
         return lib.aimet_b200_int4_linear(w, x, ldx, None, y, ldy, tokens, code, None)
 
     for kw, code, text in (({"block": 48}, _lib.AB_ERR_UNSUPPORTED, "storage block"), ({"block": 96}, _lib.AB_ERR_UNSUPPORTED, "storage block"),
-                           ({"scale_kind": 2}, _lib.AB_ERR_INVALID, "scale_kind"), ({"scale_kind": 1}, _lib.AB_ERR_INVALID, "row_scale"),
+                           ({"scale_kind": 2}, _lib.AB_ERR_INVALID, "scale_kind"), ({"row_scale": None}, _lib.AB_ERR_INVALID, "row_scale"),
                            ({"zero": 113}, _lib.AB_ERR_INVALID, "zero point"), ({"codes": None}, _lib.AB_ERR_INVALID, "NULL"),
                            ({"codes": one + 8}, _lib.AB_ERR_INVALID, "aligned"), ({"n": 0}, _lib.AB_ERR_INVALID, "0 x 128")):
         assert linear(weight(**kw)) == code and text in _lib.last_error(), kw
