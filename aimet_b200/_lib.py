@@ -187,7 +187,7 @@ SIGNATURES = {
     ),
     "aimet_b200_int4_codes_bytes": (_i64, [_i64, _i64]),
     "aimet_b200_int4_pack": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp]),
-    "aimet_b200_int4_linear": (_i32, [_w4, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp]),
+    "aimet_b200_int4_linear": (_i32, [_w4, _vp, _i64, _vp, _vp, _i64, _i64, _i32, _vp, _vp]),
     "aimet_b200_kv_append": (_i32, [_kvc, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _vp]),
     "aimet_b200_kv_gather": (_i32, [_kvc, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _vp]),
     "aimet_b200_kv_attention_scratch_bytes": (_i64, [_kvc, _i64, _i64, _i64, _i64, _i32]),

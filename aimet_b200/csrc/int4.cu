@@ -20,101 +20,17 @@
 // so that the matching fragment of x is one 16-byte read: lane t of a quad holds eight neighbouring
 // columns of every 32 (with blocks of 16 columns, four of every 16).
 #include <algorithm>
-#include <type_traits>
 
-#include "common.cuh"
+#include "int4.cuh"
 
 namespace ab {
 namespace {
 
-constexpr int kTileN = 16;    // output channels per tile
-constexpr int kTileK = 64;    // input channels per tile
-constexpr int kChunkK = 256;  // input channels per chunk: four tiles, 2 KB that one warp requests at once
-constexpr int kMvWarps = 8;   // warps of a matvec CTA
+constexpr int kMvWarps = 8;         // warps of a matvec CTA
 constexpr int kMvTiles = kMvWarps;  // channel tiles of a CTA: at most as many as warps, so that a warp meets two at most
-constexpr int64_t kMaxK = 1ll << 20;
 
-__host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
-// Codes [channel tile][tile of columns][lane][16 bytes]; scales (float32, or uint8 factors) and zero points
-// (int8) [channel tile][chunk][entry][channel][sub]: one entry per chunk (blocks of 256 columns or more), two
-// (128) or four (64 or fewer, with 64 / block neighbouring blocks in an entry).  What lies behind the matrix
-// is there and multiplies zeros of x.
-struct Int4View {
-    const uint4 *codes;
-    const void *scales;
-    const int8_t *zeros;  // NULL: `zero` for all
-    const float *row_scale;
-    int64_t n, k;
-    int chunks;   // per row: div_up(k, kChunkK)
-    int entries;  // per chunk: 1, 2, 4
-    float zero;
-};
-
-template <typename E> struct Pair16;
-template <> struct Pair16<__nv_bfloat16> {
-    static constexpr uint32_t kMagic = 0x43004300u;  // 128.0, 128.0
-    static constexpr float kBase = 128.f;
-    // Codes are multiplied as code / 256, which the same instruction gives: a sum of code * x must not
-    // leave float32's range where the sum of w * x, with its far smaller scale, does not.
-    static constexpr float kUnit = 1.f / 256.f;
-    static __device__ __forceinline__ uint32_t code(uint32_t v, uint32_t zero2) {  // (v - base) / 256 - z / 256
-        const uint32_t unit = 0x3b803b80u;
-        const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&v), *reinterpret_cast<const __nv_bfloat162 *>(&unit),
-                                         *reinterpret_cast<const __nv_bfloat162 *>(&zero2));
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-    static __device__ __forceinline__ uint32_t both(float v) {
-        const __nv_bfloat162 r = __float2bfloat162_rn(v);
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-    static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-    }
-};
-template <> struct Pair16<__half> {
-    static constexpr uint32_t kMagic = 0x64006400u;  // 1024.0, 1024.0
-    static constexpr float kBase = 1024.f;
-    static constexpr float kUnit = 1.f;
-    static __device__ __forceinline__ uint32_t code(uint32_t v, uint32_t zero2) {
-        const __half2 r = __hadd2(*reinterpret_cast<const __half2 *>(&v), *reinterpret_cast<const __half2 *>(&zero2));
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-    static __device__ __forceinline__ uint32_t both(float v) {
-        const __half2 r = __float2half2_rn(v);
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-    static __device__ __forceinline__ void mma_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-    }
-};
 template <typename E> struct MmaType { using T = E; };
 template <> struct MmaType<float> { using T = __nv_bfloat16; };
-
-// what turns a code in the mantissa of kBase into (u - z) * kUnit (all three steps exact)
-template <typename H> __device__ __forceinline__ uint32_t zero_pair(float z) {
-    return Pair16<H>::both(-(Pair16<H>::kBase + z) * Pair16<H>::kUnit);
-}
-// the codes of pair p (0..3) of a word as two 16-bit floats, (u - z) * kUnit
-template <typename H> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int p, uint32_t zero2) {
-    uint32_t v;
-    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(v) : "r"(word >> (4 * p)), "r"(Pair16<H>::kMagic));
-    return Pair16<H>::code(v, zero2);
-}
 
 // x = b0 + b1 + b2 exactly: three bfloat16 terms, cut off rather than rounded, of eight significant bits
 // each (terms below the smallest bfloat16 are lost, far under the product's float32 rounding).
@@ -130,25 +46,6 @@ __device__ __forceinline__ void split3(uint32_t w0, uint32_t w1, uint32_t (&b)[3
     x0 -= __uint_as_float(b[1] << 16);
     x1 -= __uint_as_float(b[1] & 0xffff0000u);
     b[2] = __byte_perm(__float_as_uint(x0), __float_as_uint(x1), 0x7632);
-}
-
-// SUB neighbouring values of type T as one register value (or vector of them)
-template <typename T, int SUB> struct Packed;
-template <> struct Packed<float, 1> { using V = float; static __device__ __forceinline__ float get(V v, int) { return v; } };
-template <> struct Packed<float, 2> { using V = float2; static __device__ __forceinline__ float get(V v, int i) { return i ? v.y : v.x; } };
-template <> struct Packed<float, 4> {
-    using V = float4;
-    static __device__ __forceinline__ float get(V v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-};
-template <> struct Packed<uint8_t, 1> { using V = uint8_t; static __device__ __forceinline__ float get(V v, int) { return (float)v; } };
-template <> struct Packed<uint8_t, 2> { using V = uint16_t; static __device__ __forceinline__ float get(V v, int i) { return (float)((v >> (8 * i)) & 0xff); } };
-template <> struct Packed<uint8_t, 4> { using V = uint32_t; static __device__ __forceinline__ float get(V v, int i) { return (float)((v >> (8 * i)) & 0xff); } };
-template <> struct Packed<int8_t, 1> { using V = int8_t; static __device__ __forceinline__ float get(V v, int) { return (float)v; } };
-template <> struct Packed<int8_t, 2> { using V = uint16_t; static __device__ __forceinline__ float get(V v, int i) { return (float)(int8_t)(v >> (8 * i)); } };
-template <> struct Packed<int8_t, 4> { using V = uint32_t; static __device__ __forceinline__ float get(V v, int i) { return (float)(int8_t)(v >> (8 * i)); } };
-
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // A CTA takes up to kMvTiles tiles of 16 channels (all of their columns), or a cluster of `split` CTAs takes
@@ -433,6 +330,10 @@ struct MatvecCall {
     cudaStream_t stream;
 };
 
+#ifndef GEMM_TOKENS
+#define GEMM_TOKENS 8
+#endif
+constexpr int kGemmTokens = GEMM_TOKENS;
 constexpr size_t kMvSmem = 218 * 1024, kMvSmemHalf = 104 * 1024;  // one CTA on an SM, two (beside 8 KB of sums each)
 
 template <typename E, int SUB, bool ZEROS, bool MULT> int launch_matvec(const MatvecCall &c) {
@@ -515,7 +416,7 @@ extern "C" int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int
 }
 
 extern "C" int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *x, int64_t ldx, const void *bias, void *y, int64_t ldy,
-                                      int64_t tokens, int io_dtype, void *stream) {
+                                      int64_t tokens, int io_dtype, int32_t *status, void *stream) {
     MatvecCall c;
     const int rc = check_weight(weight, &c.w);
     if (rc != AB_OK) return rc;
@@ -535,6 +436,25 @@ extern "C" int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *
     c.vec = aligned16(x) && weight->k * size % 16 == 0 && (ldx * size % 16 == 0 || tokens == 1);
     c.stream = static_cast<cudaStream_t>(stream);
     const bool mult = weight->scale_kind == 1;
+    // Many tokens: the tensor-core kernel, where rows of x start on 16 bytes (TMA).  float32 stays here: a
+    // weight's integer code times three bfloat16 terms is exact, a weight rounded to 16 bits would not be.
+    if (tokens > kGemmTokens && io_dtype != AB_F32 && aligned16(x) && ldx * size % 16 == 0) {
+        if (!status) return fail(AB_ERR_INVALID, "status is NULL");
+        Int4Gemm q;
+        q.w = c.w;
+        q.x = x;
+        q.bias = bias;
+        q.y = y;
+        q.ldx = ldx;
+        q.ldy = ldy;
+        q.tokens = (int)tokens;
+        q.block = weight->block;
+        q.io_dtype = io_dtype;
+        q.mult = mult;
+        q.status = status;
+        q.stream = c.stream;
+        return launch_int4_gemm(q);
+    }
     switch (io_dtype) {
         case AB_F32: return dispatch_matvec<float>(c, weight->block, mult);
         case AB_F16: return dispatch_matvec<__half>(c, weight->block, mult);

@@ -10,6 +10,7 @@ the reference itself only simulates them.
 
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
@@ -21,6 +22,7 @@ from ._lib import check, lib
 __all__ = ["PackedInt4Weight", "linear_int4"]
 
 _TILE_N, _TILE_K, _CHUNK_K = 16, 64, 256
+_MANY = 8  # tokens up to which the codes are multiplied exactly
 _MAX_ZERO = 112  # 16-bit floats subtract zero points up to here exactly
 
 
@@ -48,6 +50,30 @@ def _tiled(param: torch.Tensor, block: int, storage: int, in_features: int) -> t
     out = param.new_zeros(-(-n // _TILE_N) * _TILE_N, chunks * entries * sub)
     out[:n, : param.shape[1]] = param
     return out.view(-1, _TILE_N, chunks, entries, sub).permute(0, 2, 3, 1, 4).contiguous()
+
+
+class _Status:
+    """The word that a kernel's bounded waits write when they give up, per device, in pinned host memory:
+    looked at by the next call without waiting for the device."""
+
+    def __init__(self):
+        self._words: dict[int, tuple[torch.Tensor, ctypes.c_int32]] = {}
+
+    def pointer(self, device: torch.device) -> int:
+        index = device.index if device.index is not None else torch.cuda.current_device()
+        held = self._words.get(index)
+        if held is None:
+            word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+            held = self._words[index] = (word, ctypes.c_int32.from_address(word.data_ptr()))
+        word, value = held
+        if value.value:
+            code, value.value = value.value, 0
+            raise RuntimeError(f"aimet_b200: an earlier linear_int4 call on cuda:{index} gave up waiting (device status {code}); "
+                               "its output is not valid")
+        return word.data_ptr()
+
+
+_status = _Status()
 
 
 class PackedInt4Weight:
@@ -209,13 +235,16 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
     if tokens == 0:
         return out
     x = input.reshape(tokens, weight.in_features)
-    if x.stride(1) != 1 and weight.in_features > 1:
+    size = x.element_size()
+    if x.stride(1) != 1 or (tokens > 1 and x.stride(0) < weight.in_features):  # rows that overlap: an expanded input
         x = x.contiguous()
-    ldx = x.stride(0)
-    if tokens > 1 and ldx < weight.in_features:  # rows that overlap (an expanded input)
-        x = x.contiguous()
-        ldx = weight.in_features
+    status = None
+    if tokens > _MANY and size == 2:
+        status = _status.pointer(input.device)
+        if x.data_ptr() % 16 or x.stride(0) % 8:  # the tensor-core kernel wants rows that start on 16 bytes
+            padded = x.new_empty(tokens, -(-weight.in_features // 8) * 8)[:, : weight.in_features]
+            x = padded.copy_(x)
     with _lib.on_device(input.device):
-        check(lib.aimet_b200_int4_linear(weight._desc, x.data_ptr(), ldx, None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
-                                         weight.out_features, tokens, code, _lib.stream_ptr(input.device)))
+        check(lib.aimet_b200_int4_linear(weight._desc, x.data_ptr(), x.stride(0), None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
+                                         weight.out_features, tokens, code, status, _lib.stream_ptr(input.device)))
     return out

@@ -417,9 +417,12 @@ int64_t aimet_b200_int4_codes_bytes(int64_t n, int64_t k);
  * ab_int4_weight (blocks of 16 have a column order of their own) */
 int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int qmin, int block, void *out, void *stream);
 /* y[m][i] = sum_j x[m][j] * w[i][j] + bias[i] for `tokens` rows; x rows are ldx elements apart, y rows
- * ldy; bias (io_dtype, n elements) may be NULL.  Float32 accumulation, one rounding to io_dtype. */
+ * ldy; bias (io_dtype, n elements) may be NULL.  Float32 accumulation, one rounding to io_dtype.  Few
+ * tokens, float32, and rows of x that do not start on 16 bytes: codes are multiplied exactly.  Otherwise
+ * a tensor-core kernel multiplies weights rounded to io_dtype; *status (int32 that the device can write,
+ * may be pinned host memory) becomes non-zero if one of its bounded waits gives up. */
 int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *x, int64_t ldx, const void *bias, void *y,
-                           int64_t ldy, int64_t tokens, int io_dtype, void *stream);
+                           int64_t ldy, int64_t tokens, int io_dtype, int32_t *status, void *stream);
 
 /* ------------------------------------------------------------------------- *
  * A paged key / value cache in 8-bit codes and attention over it.  No counterpart in the

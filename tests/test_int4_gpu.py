@@ -78,7 +78,7 @@ def test_matches_the_product_in_64_bits(dtype, grid, tokens, n, k, block):
     bias = torch.randn(n, generator=g).to(dtype).cuda() if tokens % 2 else None
     got = linear_int4(x, packed_of(*parts), bias)
     assert got.shape == (tokens, n) and got.dtype == dtype
-    assert_close(got, x, dequantized(codes, scale, offset, int_scale), bias, weight_in_16=tokens > 16 and dtype != torch.float32)
+    assert_close(got, x, dequantized(codes, scale, offset, int_scale), bias, weight_in_16=tokens > 8 and dtype != torch.float32)
 
 
 # many tokens: whole tiles and ragged ones, odd columns, every block class
@@ -108,7 +108,7 @@ def test_strides_alignment_and_leading_dims(dtype, tokens):
     base = torch.randn(tokens, 600, device="cuda").to(dtype)
     for x in (base[:, :256], base[:, 1:257], base[:, 3:259], base.t()[:256].t().contiguous().t().contiguous().t(),
               base[:1, :256].expand(tokens, 256), base[::2, 8:264]):
-        assert_close(linear_int4(x, p), x, w, weight_in_16=x.shape[0] > 16 and dtype != torch.float32)
+        assert_close(linear_int4(x, p), x, w, weight_in_16=x.shape[0] > 8 and dtype != torch.float32)
     x = base[:2, :512].reshape(2, 2, 256)
     assert linear_int4(x, p).shape == (2, 2, 48)
     assert_close(linear_int4(x, p), x, w)

@@ -49,7 +49,7 @@ def test_entry_points_refuse_before_touching_the_device():
         return w
 
     def linear(w, x=one, y=one, ldx=128, ldy=32, tokens=2, code=_lib.AB_BF16):
-        return lib.aimet_b200_int4_linear(w, x, ldx, None, y, ldy, tokens, code, None)
+        return lib.aimet_b200_int4_linear(w, x, ldx, None, y, ldy, tokens, code, None, None)
 
     for kw, code, text in (({"block": 48}, _lib.AB_ERR_UNSUPPORTED, "storage block"), ({"block": 96}, _lib.AB_ERR_UNSUPPORTED, "storage block"),
                            ({"scale_kind": 2}, _lib.AB_ERR_INVALID, "scale_kind"), ({"row_scale": None}, _lib.AB_ERR_INVALID, "row_scale"),
@@ -62,6 +62,7 @@ def test_entry_points_refuse_before_touching_the_device():
     assert linear(weight(), code=_lib.AB_F64) == _lib.AB_ERR_UNSUPPORTED
     assert linear(weight(), x=None) == _lib.AB_ERR_INVALID
     assert linear(weight(), tokens=0, x=None, y=None) == _lib.AB_OK
+    assert linear(weight(), tokens=200) == _lib.AB_ERR_INVALID and "status" in _lib.last_error()
 
     def cache(**kw):
         c = _lib.KVCache(one, one, one, one, 10, 2, 16, 64, 0)
