@@ -330,24 +330,23 @@ struct MatvecCall {
     cudaStream_t stream;
 };
 
-#ifndef GEMM_TOKENS
-#define GEMM_TOKENS 8
-#endif
-constexpr int kGemmTokens = GEMM_TOKENS;
 constexpr size_t kMvSmem = 218 * 1024, kMvSmemHalf = 104 * 1024;  // one CTA on an SM, two (beside 8 KB of sums each)
+
+// bytes of x of one token in shared memory, and tokens that are multiplied in one pass over the weights (a
+// second pass finds them in L2): eight, or what leaves room for a second CTA on the SM
+size_t row_bytes(const Int4View &w, int io_dtype) { return (size_t)(io_dtype == AB_F32 ? 3 : 1) * (w.chunks * (kChunkK * 2) + 64); }
+int pass_tokens(size_t row) { return (int)std::min<size_t>(8, std::max<size_t>(1, kMvSmemHalf / row)); }
 
 template <typename E, int SUB, bool ZEROS, bool MULT> int launch_matvec(const MatvecCall &c) {
     const auto kernel = k_matvec<E, SUB, ZEROS, MULT>;
-    const size_t row = (size_t)(sizeof(E) == 4 ? 3 : 1) * (c.w.chunks * (kChunkK * 2) + 64);  // x of a token
+    const size_t row = row_bytes(c.w, sizeof(E) == 4 ? AB_F32 : AB_F16);
     if (row > kMvSmem)
         return fail(AB_ERR_UNSUPPORTED, "%lld input channels: x of one token does not fit shared memory", (long long)c.w.k);
     const int rc = opt_in_smem<k_matvec<E, SUB, ZEROS, MULT>>(kMvSmem);
     if (rc != AB_OK) return rc;
     const int64_t tiles = div_up(c.w.n, kTileN);
     const int sms = sm_count();
-    // Tokens that are multiplied in one pass over the weights (a second pass finds them in L2): eight, or what
-    // leaves room for a second CTA on the SM.
-    int pass = (int)std::min<size_t>(8, std::max<size_t>(1, kMvSmemHalf / row));
+    int pass = pass_tokens(row);
     pass = (int)div_up(c.tokens, div_up(c.tokens, pass));
 
     constexpr int kMost = 65535;  // passes of one launch: the grid's second dim
@@ -436,9 +435,11 @@ extern "C" int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *
     c.vec = aligned16(x) && weight->k * size % 16 == 0 && (ldx * size % 16 == 0 || tokens == 1);
     c.stream = static_cast<cudaStream_t>(stream);
     const bool mult = weight->scale_kind == 1;
-    // Many tokens: the tensor-core kernel, where rows of x start on 16 bytes (TMA).  float32 stays here: a
-    // weight's integer code times three bfloat16 terms is exact, a weight rounded to 16 bits would not be.
-    if (tokens > kGemmTokens && io_dtype != AB_F32 && aligned16(x) && ldx * size % 16 == 0) {
+    // More tokens than two passes over the weights take: the tensor-core kernel, where rows of x start on 16
+    // bytes (TMA).  Measured, 14336 x 4096: 16 tokens in two passes 19 us, on the tensor cores 29 us; 24 tokens 36
+    // and 29 us; 4096 x 14336, where x of three tokens fits: 16 tokens 67 and 31 us.  float32 stays here:
+    // a weight's integer code times three bfloat16 terms is exact, a weight rounded to 16 bits would not be.
+    if (tokens > 2 * pass_tokens(row_bytes(c.w, io_dtype)) && io_dtype != AB_F32 && aligned16(x) && ldx * size % 16 == 0) {
         if (!status) return fail(AB_ERR_INVALID, "status is NULL");
         Int4Gemm q;
         q.w = c.w;

@@ -11,13 +11,13 @@
 //
 // Orientation: weights are the M operand (128 output channels = 128 lanes of tensor memory), tokens the N
 // operand (`bn` = 32 .. 256 columns).  A stage holds 64 input channels: x comes by TMA, the weights are
-// converted by eight warps, one for each 16-channel tile of the packed layout, which store them in
+// converted, a warp for each 16-channel tile of the packed layout, and stored in
 // the 128-byte-swizzled order that tcgen05.mma reads: a lane's eight neighbouring columns are one 16-byte
-// store, and lanes of odd channels store their two halves in the other order so that eight lanes
-// meet no bank twice.  Per stage of 256 tokens the MMAs take 524 clocks, the conversion about 300 issue
+// store.  Per stage of 256 tokens the MMAs take 524 clocks, the conversion about 300 issue
 // slots of an SM's four schedulers: the tensor cores are the limit.
 //
-// Roles (512 threads): warp 0 TMA, warp 1 TMEM and MMA issue, warps 4-11 conversion, warps 12-15 epilogue.
+// Roles (768 threads): warp 0 TMA, warp 1 TMEM and MMA issue, warps 4-19 conversion (sixteen, in two turns: a
+// warp's chain of a stage, from the barrier to the fence, is long), warps 20-23 epilogue.
 // Two accumulators in tensor memory, so the epilogue of a tile runs under the MMAs of the next (one CTA per
 // SM walks the tiles).  Few tiles: a cluster of `split` CTAs shares the columns of a tile, and
 // adds its accumulators up through distributed shared memory in a fixed order.
@@ -32,11 +32,12 @@
 namespace ab {
 namespace {
 
-constexpr int kThreads4 = 512;
+constexpr int kConvWarps = 8, kConvTurns = 2;  // a channel tile each; the turns take alternate stages
+constexpr int kEpiWarp = 4 + kConvWarps * kConvTurns;  // first epilogue warp
+constexpr int kThreads4 = 32 * (kEpiWarp + 4);
 constexpr int kChannels = 128;                 // per tile
 constexpr uint32_t kWeightBytes = kChannels * 128;  // of a stage
 constexpr int kMostStages = 8;
-constexpr int kConvWarps = 8;
 enum { ST4_PRODUCER = 1, ST4_MMA = 2, ST4_CONVERT = 3, ST4_EPILOGUE = 4 };
 
 struct GemmArgs {
@@ -170,72 +171,82 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
             if (ok && elect_one()) umma_commit(bar_acc_full + 8 * buf);
             __syncwarp();
         }
-    } else if (warp >= 4 && warp < 4 + kConvWarps) {
-        const int g = lane >> 2, t = lane & 3;
+    } else if (warp >= 4 && warp < kEpiWarp) {
+        const int g = lane >> 2, t = lane & 3, mine = (warp - 4) % kConvWarps, turn = (warp - 4) / kConvWarps;
         const int64_t row_tiles = div_up(a.w.n, kTileN);
+        // of a chunk's four column tiles this warp converts `turn` and `turn + 2`
         struct {
-            uint4 code[4];
-            typename SP::V scale[4][2];
-            typename ZP::V zero[4][2];
+            uint4 code[2];
+            typename SP::V scale[2][2];
+            typename ZP::V zero[2][2];
         } buf[2];
-        const int off[4] = {0, a.w.entries / 4 * kTileN, a.w.entries / 2 * kTileN, a.w.entries * 3 / 4 * kTileN};
-        auto load = [&](int b, int tile, int c) {
-            const int64_t row = (int64_t)(tile % a.n_ct) * (kChannels / kTileN) + warp - 4;
-            if (row >= row_tiles) return;  // channels behind the matrix: any finite weights, nobody stores their sums
-            const uint4 *code = a.w.codes + (row * a.w.chunks + c) * 128 + lane;
-            const int64_t entry = (row * a.w.chunks + c) * a.w.entries * kTileN + g;
-            const auto *scale = static_cast<const typename SP::V *>(a.w.scales) + entry;
-            const auto *zero = reinterpret_cast<const typename ZP::V *>(a.w.zeros) + (ZEROS ? entry : 0);
+        // the next chunk to request
+        int req_tile = worker, req_c = c0;
+        bool inside;  // channels behind the matrix: any finite weights, nobody stores their sums
+        const uint4 *code_at;
+        const typename SP::V *scale_at;
+        const typename ZP::V *zero_at;
+        auto seek = [&]() {
+            const int64_t row = (int64_t)(req_tile % a.n_ct) * (kChannels / kTileN) + mine;
+            inside = row < row_tiles && req_tile < total;
+            const int64_t chunk = row * a.w.chunks + c0, entry = chunk * a.w.entries * kTileN + g;
+            code_at = a.w.codes + chunk * 128 + 32 * turn + lane;
+            scale_at = static_cast<const typename SP::V *>(a.w.scales) + entry;
+            zero_at = reinterpret_cast<const typename ZP::V *>(a.w.zeros) + (ZEROS ? entry : 0);
+        };
+        seek();
+        const int off[2] = {a.w.entries * turn / 4 * kTileN, a.w.entries * (turn + 2) / 4 * kTileN}, step = a.w.entries * kTileN;
+        auto load = [&](int b) {
+            if (inside) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                buf[b].code[i] = code[32 * i];
+                for (int i = 0; i < 2; ++i) {
+                    buf[b].code[i] = code_at[64 * i];
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int at = (SUB == 1 ? off[i] : kTileN * i) + 8 * r;
-                    buf[b].scale[i][r] = scale[at];
-                    if constexpr (ZEROS) buf[b].zero[i][r] = zero[at];
+                    for (int r = 0; r < 2; ++r) {
+                        buf[b].scale[i][r] = scale_at[off[i] + 8 * r];
+                        if constexpr (ZEROS) buf[b].zero[i][r] = zero_at[off[i] + 8 * r];
+                    }
                 }
+            }
+            code_at += 128;
+            scale_at += step;
+            zero_at += ZEROS ? step : 0;
+            if (++req_c == c1) {
+                req_c = c0;
+                req_tile += workers;
+                seek();
             }
         };
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 buf[b].code[i] = make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) buf[b].scale[i][r] = typename SP::V{}, buf[b].zero[i][r] = typename ZP::V{};
             }
         const uint32_t one_zero = zero_pair<E>(a.w.zero);
-        const bool odd = g & 1;
-        const uint32_t row_at = (16 * (warp - 4) + g) * 128;  // and + 1024 for channel g + 8
-        int stage = 0;
+        const uint32_t row_at = (16 * mine + g) * 128;  // and + 1024 for channel g + 8
+        int stage = 0, at = 0;  // the stage of column tile `at`, counted over all tiles of this CTA
         uint32_t phase = 0;
         bool ok = true;
-        // the next chunk to request
-        int req_tile = worker, req_c = c0;
-        auto advance = [&]() {
-            if (++req_c == c1) req_c = c0, req_tile += workers;
-        };
         // weights are never written by a kernel that lets its successor start early: before the wait
-        load(0, req_tile, req_c);
-        advance();
+        load(0);
         pdl_wait();
-        for (int tile = worker; ok && tile < total; tile += workers) {
+        int first = -kt0;  // what is added to a column tile's index to count it over all tiles of this CTA
+        for (int tile = worker; ok && tile < total; tile += workers, first += kt1 - kt0) {
             for (int c = c0; ok && c < c1; c += 2) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b) {
                     if (c + b >= c1 || !ok) break;
-                    if (req_tile < total) {
-                        load(b ^ 1, req_tile, req_c);
-                        advance();
-                    }
+                    load(b ^ 1);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (4 * (c + b) + i >= kt1 || !ok) break;
+                    for (int i = 0; i < 2; ++i) {
+                        const int kt = 4 * (c + b) + turn + 2 * i;
+                        if (kt >= kt1) break;
                         const uint4 w4 = buf[b].code[i];
-                        // lanes of odd channels store their second half first
-                        const uint32_t word[4] = {odd ? w4.z : w4.x, odd ? w4.w : w4.y, odd ? w4.x : w4.z, odd ? w4.y : w4.w};
-                        uint32_t out[2][2][4];  // [half stored first, second][channel g, g + 8][pairs]
+                        const uint32_t word[4] = {w4.x, w4.y, w4.z, w4.w};
+                        uint32_t out[2][2][4];  // [half of the columns][channel g, g + 8][pairs]
 #pragma unroll
                         for (int r = 0; r < 2; ++r)
 #pragma unroll
@@ -243,17 +254,9 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
 #pragma unroll
                                 for (int p = 0; p < 4; ++p) {
                                     const int q = 2 * e + r;
-                                    // the block of these columns within the tile: first half of the tile or second, and with
-                                    // blocks of 16 first half of that or second
-                                    const int s0 = SUB == 1 ? 0 : SUB == 2 ? e : 2 * e + (p >> 1), s1 = SUB == 1 ? 0 : SUB == 2 ? 1 - e : 2 * (1 - e) + (p >> 1);
-                                    float f = SP::get(buf[b].scale[i][r], s0);
-                                    if (SUB > 1 && odd) f = SP::get(buf[b].scale[i][r], s1);
-                                    uint32_t z = one_zero;
-                                    if constexpr (ZEROS) {
-                                        float zf = ZP::get(buf[b].zero[i][r], s0);
-                                        if (SUB > 1 && odd) zf = ZP::get(buf[b].zero[i][r], s1);
-                                        z = zero_pair<E>(zf);
-                                    }
+                                    const int sub = SUB == 1 ? 0 : SUB == 2 ? e : 2 * e + (p >> 1);  // the columns' block within the tile
+                                    const float f = SP::get(buf[b].scale[i][r], sub);
+                                    const uint32_t z = ZEROS ? zero_pair<E>(ZP::get(buf[b].zero[i][r], sub)) : one_zero;
                                     const uint32_t v = code_pair<E>(word[q], p, z), hi = Pair16<E>::both(f);
                                     if (MULT) {
                                         out[e][r][p] = mul2(v, hi, E());
@@ -262,34 +265,35 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
                                         out[e][r][p] = fma2(v, hi, mul2(v, lo, E()), E());
                                     }
                                 }
+                        stage += first + kt - at;  // at most three further: fewer than there are stages
+                        at = first + kt;
+                        if (stage >= a.stages) stage -= a.stages, phase ^= 1;
                         ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, a.status, ST4_CONVERT, a.timeout_ns);
                         ok = __all_sync(0xffffffffu, ok);
                         if (!ok) break;
                         uint8_t *dst = ring + (size_t)stage * stage_bytes + row_at;
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const int h = e ^ (int)odd;
 #pragma unroll
                             for (int r = 0; r < 2; ++r) {
                                 const uint32_t *v = out[e][r];
                                 if constexpr (SUB == 4) {  // four columns at 32 h + 4 t and four at 32 h + 16 + 4 t
-                                    *reinterpret_cast<uint2 *>(dst + 1024 * r + (((4 * h + (t >> 1)) ^ g) << 4) + 8 * (t & 1)) = make_uint2(v[0], v[1]);
-                                    *reinterpret_cast<uint2 *>(dst + 1024 * r + (((4 * h + 2 + (t >> 1)) ^ g) << 4) + 8 * (t & 1)) = make_uint2(v[2], v[3]);
+                                    *reinterpret_cast<uint2 *>(dst + 1024 * r + (((4 * e + (t >> 1)) ^ g) << 4) + 8 * (t & 1)) = make_uint2(v[0], v[1]);
+                                    *reinterpret_cast<uint2 *>(dst + 1024 * r + (((4 * e + 2 + (t >> 1)) ^ g) << 4) + 8 * (t & 1)) = make_uint2(v[2], v[3]);
                                 } else {
-                                    *reinterpret_cast<uint4 *>(dst + 1024 * r + (((4 * h + t) ^ g) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+                                    *reinterpret_cast<uint4 *>(dst + 1024 * r + (((4 * e + t) ^ g) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
                                 }
                             }
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) mbar_arrive(bar_full + 8 * stage);
-                        if (++stage == a.stages) stage = 0, phase ^= 1;
                     }
                 }
             }
             if ((c1 - c0) & 1) buf[0] = buf[1];  // the tile ended on the first buffer: the next one starts there again
         }
-    } else if (warp >= 12) {
+    } else if (warp >= kEpiWarp) {
         pdl_wait();
         const int quad = warp & 3;
         uint32_t pass = 0;

@@ -22,7 +22,6 @@ from ._lib import check, lib
 __all__ = ["PackedInt4Weight", "linear_int4"]
 
 _TILE_N, _TILE_K, _CHUNK_K = 16, 64, 256
-_MANY = 8  # tokens up to which the codes are multiplied exactly
 _MAX_ZERO = 112  # 16-bit floats subtract zero points up to here exactly
 
 
@@ -239,9 +238,9 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
     if x.stride(1) != 1 or (tokens > 1 and x.stride(0) < weight.in_features):  # rows that overlap: an expanded input
         x = x.contiguous()
     status = None
-    if tokens > _MANY and size == 2:
+    if tokens > 2 and size == 2:  # the library may choose its tensor-core kernel, which has bounded waits
         status = _status.pointer(input.device)
-        if x.data_ptr() % 16 or x.stride(0) % 8:  # the tensor-core kernel wants rows that start on 16 bytes
+        if tokens > 16 and (x.data_ptr() % 16 or x.stride(0) % 8):  # it tensor-core kernel wants rows that start on 16 bytes
             padded = x.new_empty(tokens, -(-weight.in_features // 8) * 8)[:, : weight.in_features]
             x = padded.copy_(x)
     with _lib.on_device(input.device):
