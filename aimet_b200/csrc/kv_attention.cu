@@ -6,10 +6,13 @@
 // maximum and sum of the softmax; the codes go from HBM to the operand registers in 8 bits.
 //
 // What bounds it is reading the codes: 2 * dim bytes per token and head, for a handful of rows (the
-// query heads that share a head of the cache, times the query tokens).  Those rows are one 16-row tile
-// of mma.sync (tcgen05 needs 64 rows at least, and here the tensor cores are not the limit): scores =
-// Q (16 x dim) . K^T, then O (16 x dim) += P (16 x tokens) . V.  Codes become float16 pairs exactly (a
-// byte permute puts code + 128 into the mantissa of 1024, subtracting 1152 leaves the code).  The scales
+// query heads that share a head of the cache, times the query tokens); at the measured copy rate an SM gets 23
+// codes per clock, so what has to be saved is instructions per code.  The codes are the 16-row operand of
+// mma.sync and eight query rows the 8 columns (tcgen05 needs 128 rows of converted codes in shared
+// memory first): S^T (16 tokens x 8) = K . Q^T, then O^T (dim x 8) += V^T . P^T.  Codes become float16 pairs
+// exactly (a byte permute puts code + 128 into the mantissa of 1024, subtracting 1152 leaves the code), P^T
+// moves from the first product's result layout to the second's operand layout by an 8 x 8 transpose
+// (movmatrix).  More rows are further columns that share the converted codes.  The scales
 // never touch an element: a tile of 16 tokens lies in one page, so the key scale multiplies the scores,
 // and log2 of the value scale is added to the exponent of the weights that multiply V.
 //
@@ -38,7 +41,13 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStages = 4;
 constexpr int kTokens = 16;     // per tile
-constexpr int kMinPiece = 128;  // tokens a CTA gets at least: two tiles per warp
+// Tokens of a piece at least: two tiles per warp where contexts are short (one of 500 tokens: 8.2 us with pieces
+// of 128, 9.5 with 256, 9.2 uncut), up to 512 where they are long and joining many pieces would cost more
+// than it gains (8000 tokens: 13.8 us with 512, 15.2 with 192).
+constexpr int kMinPiece = 128, kMaxMinPiece = 512;
+// Pieces per CTA slot of the machine: one where pieces are all that fills it (two of 131072 tokens: 108 us, 119 with
+// two); three where sequences and heads do, so that ragged lengths even out (64 of 1000 to 4000: 99 us, 106 with one).
+constexpr int kWaves = 3;
 
 struct AttnArgs {
     const int8_t *key, *value;
@@ -52,6 +61,7 @@ struct AttnArgs {
     float *part;       // partial results of the pieces, or NULL
     const int32_t *table, *context, *qlens;
     int64_t table_stride;
+    uint32_t page_magic;  // tile / (page / kTokens) == umulhi(tile, page_magic) (tiles below 2^26, at most 64 in a page); 0: one tile in a page
     int table_width, seqs, tokens, group, row_blocks, pieces;
     int causal, window, vec;
     int target;        // CTAs per head and row block that fill the machine
@@ -97,9 +107,15 @@ __device__ __forceinline__ uint32_t unbias(uint32_t v) {
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
 // Shared memory of a tile: rows of DP bytes, cut into 16-byte chunks whose place within a 128-byte line is
 // permuted so that the operand reads below meet no bank twice.  K is read 16 bytes per lane, eight lanes
-// at a time from two neighbouring rows; V four bytes per lane from four rows two apart.
+// at a time from two neighbouring rows; V eight bytes per lane, sixteen lanes at a time from four rows two apart.
 template <int DP> __device__ __forceinline__ uint32_t place_k(int row, int chunk) {
     const uint32_t at = row * DP + chunk * 16;
     return DP == 64 ? at : at ^ ((row & 1) << 6);
@@ -128,6 +144,19 @@ template <typename E> __device__ __forceinline__ void load_row16(const E *p, int
             for (int i = 0; i < V; ++i) v.v[i] = p[j * V + i];
 #pragma unroll
         for (int i = 0; i < V; ++i) f[j * V + i] = to_f32(v.v[i]);
+    }
+}
+
+// four neighbouring results, scaled (dims are multiples of 16 and outputs 16-byte aligned)
+template <typename E> __device__ __forceinline__ void store4(E *dst, const float4 &v, float inv, bool dead) {
+    const float e[4] = {dead ? 0.f : v.x * inv, dead ? 0.f : v.y * inv, dead ? 0.f : v.z * inv, dead ? 0.f : v.w * inv};
+    if constexpr (sizeof(E) == 4) {
+        *reinterpret_cast<float4 *>(dst) = make_float4(e[0], e[1], e[2], e[3]);
+    } else {
+        E h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = Cvt<float, E>::store(e[j]);
+        *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(h);
     }
 }
 
@@ -165,22 +194,24 @@ __device__ __forceinline__ int piece_tokens(const AttnArgs &a, int lane) {
         most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     }
     long long n = max((sum + a.target - 1) / a.target, ((long long)most + a.pieces - 1) / a.pieces);
-    n = max(n, (long long)kMinPiece);
+    n = max(n, (long long)min(max(most / 16, kMinPiece), kMaxMinPiece));
     return (int)((n + 63) / 64 * 64);
 }
 
-template <typename E, int DP, int RT> struct Layout {
-    static constexpr int kTile = kTokens * DP;             // bytes of K or V of a tile
-    static constexpr int kStage = 2 * kTile + 128;          // and the two scales, padded to a swizzle line
+template <typename E, int DP, int NQ> struct Layout {
+    static constexpr int kTile = kTokens * DP;              // bytes of K or V of a tile
+    static constexpr int kStage = 2 * kTile + 128;           // and the two scales, padded to a swizzle line
     static constexpr int kWarp = kStages * kStage;
-    static constexpr int kRows = 16 * RT;
+    static constexpr int kRows = 8 * NQ;                     // query rows of a CTA
     static constexpr int kJoin = kRows * DP * 4 + kRows * 8;  // a warp's O, maxima and sums
     static constexpr int kPerWarp = kWarp > kJoin ? kWarp : (kJoin + 127) / 128 * 128;
     static constexpr int kSmem = kWarps * kPerWarp;
 };
 
-template <typename E, int DP, int RT> __global__ void __launch_bounds__(kWarps * 32) k_kv_attention(AttnArgs a) {
-    using L = Layout<E, DP, RT>;
+// FULL: the head's dim is DP, a constant
+template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds__(kWarps * 32) k_kv_attention(AttnArgs a) {
+    if (FULL) a.dim = DP;
+    using L = Layout<E, DP, NQ>;
     constexpr bool F32 = sizeof(E) == 4;
     constexpr int NC = DP / 64;       // 64-wide parts of a row
     constexpr int QS = F32 ? 2 : 1;   // float16 terms of q and of the weights
@@ -198,91 +229,15 @@ template <typename E, int DP, int RT> __global__ void __launch_bounds__(kWarps *
     const int first_token = row0 / a.group, last_token = (row0 + live - 1) / a.group;
     Span span = {0, 0};
     if (live > 0) span = span_of(a, ctx, len, first_token, last_token);
-    int from = span.lo, to = span.hi;
+    int from = span.lo, to = span.hi, count = 1;  // pieces of this row block
     if (a.part) {
         const int n = piece_tokens(a, lane);
         const int start = span.lo & ~(kTokens - 1);
         const long long p0 = (long long)start + (long long)piece * n;
         from = (int)min((long long)to, max((long long)from, p0));
         to = (int)min((long long)to, p0 + n);
-        if (piece > 0 && from >= to) return;  // the joining kernel derives the same pieces
-    }
-
-    // the queries of this warp's rows as operand fragments
-    uint32_t qf[RT][QS][NC][4][4];
-    float score_scale[RT][2];
-    int lo_row[RT][2], hi_row[RT][2];
-    int max_lo = 0, min_hi = 0x7fffffff;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = 16 * rt + g + 8 * i;
-            const bool alive = r < live;
-            const int token = alive ? (row0 + r) / a.group : first_token;
-            const int gq = alive ? (row0 + r) % a.group : 0;
-            const Span sp = live > 0 ? span_of(a, ctx, len, token, token) : Span{0, 0};
-            lo_row[rt][i] = sp.lo;
-            hi_row[rt][i] = sp.hi;
-            const E *p = static_cast<const E *>(a.q) + (int64_t)s * a.q_seq + (int64_t)token * a.q_tok + (int64_t)(h * a.group + gq) * a.q_head;
-            float top = 0.f;
-            float f[NC][16];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const int d = 64 * c + 16 * t;
-                load_row16(p + d, alive ? a.dim - d : 0, a.vec, f[c]);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(f[c][e]));
-            }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // top in [2^(e-1), 2^e): times 2^(15-e) it lies in [2^14, 2^15)
-            int e = 0;
-            float up = 1.f, down = 1.f;
-            if (top > 0.f && top <= 3.402823466e38f) {
-                frexpf(top, &e);
-                e = min(max(15 - e, -120), 120);
-                up = ldexpf(1.f, e);
-                down = ldexpf(1.f, -e);
-            }
-            score_scale[rt][i] = down * a.scale_log2;
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int st = 0; st < 4; ++st)
-#pragma unroll
-                    for (int p2 = 0; p2 < 2; ++p2) {
-                        const float x0 = f[c][4 * st + 2 * p2] * up, x1 = f[c][4 * st + 2 * p2 + 1] * up;
-                        const uint32_t hi = half2_of(x0, x1);
-                        qf[rt][0][c][st][i + 2 * p2] = hi;
-                        if constexpr (F32) {
-                            const float2 b = floats_of(hi);
-                            qf[rt][QS - 1][c][st][i + 2 * p2] = half2_of(x0 - b.x, x1 - b.y);
-                        }
-                    }
-        }
-    }
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) max_lo = max(max_lo, lo_row[rt][i]), min_hi = min(min_hi, hi_row[rt][i]);
-    // of all rows of the tile, so that the choice of the masked path is the warp's
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        max_lo = max(max_lo, __shfl_xor_sync(0xffffffffu, max_lo, o));
-        min_hi = min(min_hi, __shfl_xor_sync(0xffffffffu, min_hi, o));
-    }
-
-    float m[RT][2], mv[RT][2], sum[RT][2];
-    float o[RT][DP / 8][4];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) m[rt][i] = mv[rt][i] = -CUDART_INF_F, sum[rt][i] = 0.f;
-#pragma unroll
-        for (int n = 0; n < DP / 8; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[rt][n][i] = 0.f;
+        if (piece > 0 && from >= to) return;
+        count = max(1, (span.hi - start + n - 1) / n);
     }
 
     const int tile0 = from / kTokens, tiles = from < to ? (to - 1) / kTokens - tile0 + 1 : 0;
@@ -290,166 +245,245 @@ template <typename E, int DP, int RT> __global__ void __launch_bounds__(kWarps *
     uint8_t *ring = smem + warp * L::kPerWarp;
     const uint32_t ring_at = smem_u32(ring);
     const int32_t *table = a.table + (int64_t)s * a.table_stride;
-    const int chunks = a.dim / 16;
 
-    auto page_of = [&](int i) -> int {  // of this warp's i-th tile; to <= table_width * page
-        return i < mine ? table[(int64_t)(tile0 + warp + i * kWarps) * kTokens / a.page] : -1;
+    // What a lane copies of every tile: 16-byte chunk lane % CH of rows lane / CH, lane / CH + 32 / CH, ...; chunks
+    // beyond the head's dim are filled with zeros.
+    constexpr int CH = DP / 16, STEP = 32 / CH, COPIES = kTokens / STEP;
+    const int copy_row = lane / CH, copy_chunk = lane % CH;
+    const bool copies = copy_chunk * 16 < a.dim;
+    const int64_t copy_off = copies ? (int64_t)copy_row * a.dim + copy_chunk * 16 : 0;
+    const int copy_step = copies ? STEP * a.dim : 0;
+    // page and place in it of this warp's i-th tile; to <= table_width * page, and -1 is no page
+    const uint32_t per_page = a.page / kTokens;
+    struct Where {
+        int page;
+        uint32_t in_page;
     };
-    auto request = [&](int i, int pg) {
+    auto where = [&](int i) -> Where {
+        const uint32_t tile = tile0 + warp + i * kWarps, block = a.page_magic ? __umulhi(tile, a.page_magic) : tile;
+        return {i < mine ? table[block] : -1, tile - block * per_page};
+    };
+    uint32_t gone = 0;  // bit per stage: its tile has no page
+    const int64_t page_bytes = (int64_t)a.page * a.dim;
+    const int8_t *key = a.key + h * page_bytes + copy_off, *value = a.value + h * page_bytes + copy_off;
+    const float *scale = (lane ? a.value_scale : a.key_scale) + h;  // lanes 0 and 1 copy the scales
+    const int tile_bytes = kTokens * a.dim;
+    auto request = [&](int i, const Where &w) {
+        const int slot = i % kStages;
         if (i < mine) {
-            const int token = (tile0 + warp + i * kWarps) * kTokens;
-            const bool there = pg >= 0 && pg < a.pages;
-            const int64_t ph = there ? (int64_t)pg * a.heads + h : 0;
-            const int64_t at = (ph * a.page + token % a.page) * a.dim;
-            const uint32_t dst = ring_at + (i % kStages) * L::kStage;
+            const bool there = (uint32_t)w.page < (uint32_t)a.pages;
+            const int64_t ph = there ? (int64_t)w.page * a.heads : 0;
+            const int64_t at = ph * page_bytes + w.in_page * tile_bytes;
+            const int bytes = there && copies ? 16 : 0;  // where there is no page, zeros: what page 0 holds must not reach the sums
+            const uint32_t dst = ring_at + slot * L::kStage;
+            const int8_t *kp = key + at, *vp = value + at;
+            gone = (gone & ~(1u << slot)) | (uint32_t)!there << slot;
 #pragma unroll
-            for (int c = lane; c < L::kTile / 16; c += 32) {
-                const int r = c / (DP / 16), ch = c % (DP / 16);
-                const bool ok = there && ch < chunks;
-                const int64_t off = ok ? at + (int64_t)r * a.dim + ch * 16 : 0;
-                cp_async16(dst + place_k<DP>(r, ch), a.key + off, ok ? 16 : 0);
-                cp_async16(dst + L::kTile + place_v<DP>(r, ch * 16), a.value + off, ok ? 16 : 0);
+            for (int j = 0; j < COPIES; ++j) {
+                const int r = copy_row + j * STEP;
+                cp_async16(dst + place_k<DP>(r, copy_chunk), kp + j * copy_step, bytes);
+                cp_async16(dst + L::kTile + place_v<DP>(r, copy_chunk * 16), vp + j * copy_step, bytes);
             }
-            // where there is no page, zeros: whatever page 0 holds must not reach the sums
-            if (lane == 0) cp_async4(dst + 2 * L::kTile, a.key_scale + ph, there ? 4 : 0);
-            if (lane == 1) cp_async4(dst + 2 * L::kTile + 4, a.value_scale + ph, there ? 4 : 0);
+            if (lane < 2) cp_async4(dst + 2 * L::kTile + 4 * lane, scale + ph, there ? 4 : 0);
         }
         cp_commit();
     };
+    Where next;
+    {
+        Where w[kStages];
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) w[i] = where(i);
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) request(i, w[i]);
+        next = w[kStages - 1];
+    }
 
-    int pg_of[kStages];  // pages of the tiles in flight, to know which are not there
+    // the queries as operand fragments: this lane's part of query row g of every eight
+    uint32_t qf[NQ][QS][NC][4][2];
+    float score_scale[NQ][2];             // of rows 2t, 2t + 1 of the eight, as everything below
+    int lo_row[NQ][2], hi_row[NQ][2];
+    int max_lo = 0, min_hi = 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < kStages; ++i) pg_of[i] = page_of(i);
+    for (int n = 0; n < NQ; ++n) {
+        const int r = 8 * n + g;
+        const bool alive = r < live;
+        const int token = alive ? (row0 + r) / a.group : 0, gq = alive ? (row0 + r) % a.group : 0;
+        const E *p = static_cast<const E *>(a.q) + (int64_t)s * a.q_seq + (int64_t)token * a.q_tok + (int64_t)(h * a.group + gq) * a.q_head;
+        float top = 0.f;
+        float f[NC][16];
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) request(i, pg_of[i]);
-    int pg_next = pg_of[kStages - 1];
-    uint32_t gone = 0;  // bit per stage: its tile has no page
+        for (int c = 0; c < NC; ++c) {
+            const int d = 64 * c + 16 * t;
+            load_row16(p + d, alive ? a.dim - d : 0, a.vec, f[c]);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) gone |= (uint32_t)(pg_of[i] < 0 || pg_of[i] >= a.pages) << i;
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(f[c][e]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // top in [2^(e-1), 2^e): times 2^(15-e) it lies in [2^14, 2^15)
+        int e = 0;
+        float up = 1.f, down = 1.f;
+        if (top > 0.f && top <= 3.402823466e38f) {
+            frexpf(top, &e);
+            e = min(max(15 - e, -120), 120);
+            up = ldexpf(1.f, e);
+            down = ldexpf(1.f, -e);
+        }
+        down *= a.scale_log2;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            score_scale[n][i] = __shfl_sync(0xffffffffu, down, (2 * t + i) * 4);
+            const int row = 8 * n + 2 * t + i;
+            const int tok = row < live ? (row0 + row) / a.group : first_token;
+            const Span sp = live > 0 ? span_of(a, ctx, len, tok, tok) : Span{0, 0};
+            lo_row[n][i] = sp.lo;
+            hi_row[n][i] = sp.hi;
+            max_lo = max(max_lo, sp.lo);
+            min_hi = min(min_hi, sp.hi);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int st = 0; st < 4; ++st)
+#pragma unroll
+                for (int p2 = 0; p2 < 2; ++p2) {
+                    const float x0 = f[c][4 * st + 2 * p2] * up, x1 = f[c][4 * st + 2 * p2 + 1] * up;
+                    const uint32_t hi = half2_of(x0, x1);
+                    qf[n][0][c][st][p2] = hi;
+                    if constexpr (F32) {
+                        const float2 b = floats_of(hi);
+                        qf[n][QS - 1][c][st][p2] = half2_of(x0 - b.x, x1 - b.y);
+                    }
+                }
+    }
+    // of all rows, so that the choice of the masked path is the warp's
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+        max_lo = max(max_lo, __shfl_xor_sync(0xffffffffu, max_lo, o));
+        min_hi = min(min_hi, __shfl_xor_sync(0xffffffffu, min_hi, o));
+    }
+
+    float m[NQ][2], mv[NQ][2], sum[NQ][2];
+    float o[NQ][DP / 16][4];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m[n][i] = mv[n][i] = -CUDART_INF_F, sum[n][i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[n][d][i] = 0.f;
+    }
 
     for (int i = 0; i < mine; ++i) {
         cp_wait<kStages - 2>();
         __syncwarp();
-        {
-            const int nx = i + kStages - 1, slot = nx % kStages;
-            const int after = page_of(nx + 1);
-            request(nx, pg_next);
-            gone = (gone & ~(1u << slot)) | (uint32_t)(pg_next < 0 || pg_next >= a.pages) << slot;
-            pg_next = after;
-        }
         const int slot = i % kStages;
+        const bool hole = (gone >> slot) & 1;
+        {
+            const Where after = where(i + kStages);
+            request(i + kStages - 1, next);
+            next = after;
+        }
         const uint8_t *kt = ring + slot * L::kStage, *vt = kt + L::kTile;
         const float2 scales = *reinterpret_cast<const float2 *>(kt + 2 * L::kTile);
         const int token0 = (tile0 + warp + i * kWarps) * kTokens;
 
-        // scores
-        float sc[RT][2][4];
+        // scores: tokens g and g + 8 of the tile, query rows 2t and 2t + 1
+        float sc[NQ][4];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+        for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int e = 0; e < 4; ++e) sc[n][e] = 0.f;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[rt][n][e] = 0.f;
+        for (int c = 0; c < NC; ++c) {
+            const uint4 x4 = *reinterpret_cast<const uint4 *>(kt + place_k<DP>(g, 4 * c + t));
+            const uint4 y4 = *reinterpret_cast<const uint4 *>(kt + place_k<DP>(g + 8, 4 * c + t));
+            const uint32_t x[4] = {x4.x, x4.y, x4.z, x4.w}, y[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
+            for (int st = 0; st < 4; ++st) {
+                const uint32_t u = x[st] ^ 0x80808080u, v = y[st] ^ 0x80808080u;
+                const uint32_t k[4] = {unbias(__byte_perm(u, 0x64646464u, 0x4140)), unbias(__byte_perm(v, 0x64646464u, 0x4140)),
+                                       unbias(__byte_perm(u, 0x64646464u, 0x4342)), unbias(__byte_perm(v, 0x64646464u, 0x4342))};
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const uint4 w4 = *reinterpret_cast<const uint4 *>(kt + place_k<DP>(8 * n + g, 4 * c + t));
-                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    const uint32_t u = w[st] ^ 0x80808080u;
-                    const uint32_t b0 = unbias(__byte_perm(u, 0x64646464u, 0x4140)), b1 = unbias(__byte_perm(u, 0x64646464u, 0x4342));
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int q = 0; q < QS; ++q) mma_f16(sc[rt][n], qf[rt][q][c][st], b0, b1);
-                }
+                    for (int q = 0; q < QS; ++q) mma_f16(sc[n], k, qf[n][q][c][st][0], qf[n][q][c][st][1]);
             }
+        }
 
-        const bool masked = token0 < max_lo || token0 + kTokens > min_hi || ((gone >> slot) & 1);
+        const bool masked = token0 < max_lo || token0 + kTokens > min_hi || hole;
         const float lv = scales.y > 0.f ? log2_fast(scales.y) : -CUDART_INF_F;
-        uint32_t pf[RT][QS][4];
+        uint32_t pf[NQ][QS][2];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            float p[2][2][2];  // [row][n][e]
+        for (int n = 0; n < NQ; ++n) {
             bool moved = false;
-            float turn[2];
+            float turn[2], p[2][2];  // [row][token g, g + 8]
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
-                const float f = score_scale[rt][r] * scales.x;
-                float top = -CUDART_INF_F;
+                const float f = score_scale[n][r] * scales.x;
+                float x0 = sc[n][r] * f, x1 = sc[n][2 + r] * f;
+                if (masked) {
+                    const int at = token0 + g;
+                    if (at < lo_row[n][r] || at >= hi_row[n][r] || hole) x0 = -CUDART_INF_F;
+                    if (at + 8 < lo_row[n][r] || at + 8 >= hi_row[n][r] || hole) x1 = -CUDART_INF_F;
+                }
+                float top = fmaxf(x0, x1);
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float v = sc[rt][n][2 * r + e] * f;
-                        if (masked) {
-                            const int at = token0 + 8 * n + 2 * t + e;
-                            if (at < lo_row[rt][r] || at >= hi_row[rt][r] || ((gone >> slot) & 1)) v = -CUDART_INF_F;
-                        }
-                        p[r][n][e] = v;
-                        top = fmaxf(top, v);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m1 = fmaxf(m[rt][r], top), ref = m1 == -CUDART_INF_F ? 0.f : m1;
-                float add = 0.f;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) add += exp2_fast(p[r][n][e] - ref);
-                sum[rt][r] = sum[rt][r] * exp2_fast(m[rt][r] - ref) + add;
-                m[rt][r] = m1;
-                const float v1 = fmaxf(mv[rt][r], top + lv), vref = v1 == -CUDART_INF_F ? 0.f : v1;
-                turn[r] = exp2_fast(mv[rt][r] - vref);
-                moved |= v1 != mv[rt][r];
-                mv[rt][r] = v1;
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) p[r][n][e] = exp2_fast(p[r][n][e] + (lv - vref));
+                for (int w = 4; w <= 16; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+                const float m1 = fmaxf(m[n][r], top), ref = m1 == -CUDART_INF_F ? 0.f : m1;
+                sum[n][r] = sum[n][r] * exp2_fast(m[n][r] - ref) + (exp2_fast(x0 - ref) + exp2_fast(x1 - ref));
+                m[n][r] = m1;
+                const float v1 = fmaxf(mv[n][r], top + lv), vref = v1 == -CUDART_INF_F ? 0.f : v1;
+                turn[r] = exp2_fast(mv[n][r] - vref);
+                moved |= v1 != mv[n][r];
+                mv[n][r] = v1;
+                p[r][0] = exp2_fast(x0 + (lv - vref));
+                p[r][1] = exp2_fast(x1 + (lv - vref));
             }
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int n = 0; n < DP / 8; ++n) {
-                    o[rt][n][0] *= turn[0];
-                    o[rt][n][1] *= turn[0];
-                    o[rt][n][2] *= turn[1];
-                    o[rt][n][3] *= turn[1];
+                for (int d = 0; d < DP / 16; ++d) {
+                    o[n][d][0] *= turn[0];
+                    o[n][d][1] *= turn[1];
+                    o[n][d][2] *= turn[0];
+                    o[n][d][3] *= turn[1];
                 }
             }
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const uint32_t hi = half2_of(p[r][n][0], p[r][n][1]);
-                    pf[rt][0][2 * n + r] = hi;
-                    if constexpr (F32) {
-                        const float2 b = floats_of(hi);
-                        pf[rt][QS - 1][2 * n + r] = half2_of(p[r][n][0] - b.x, p[r][n][1] - b.y);
-                    }
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t hi = half2_of(p[0][k], p[1][k]);
+                pf[n][0][k] = transpose8(hi);
+                if constexpr (F32) {
+                    const float2 b = floats_of(hi);
+                    pf[n][QS - 1][k] = transpose8(half2_of(p[0][k] - b.x, p[1][k] - b.y));
                 }
+            }
         }
 
-        // O += P . V
+        // O^T += V^T . P^T: dims 64 c + 8 g + 2 j and + 1 are rows g and g + 8 of product j
 #pragma unroll
-        for (int c = 0; c < DP / 32; ++c) {
-            uint32_t w[4];
+        for (int c = 0; c < NC; ++c) {
+            uint2 w[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                w[r] = *reinterpret_cast<const uint32_t *>(vt + place_v<DP>(2 * t + (r & 1) + 8 * (r >> 1), 32 * c + 4 * g)) ^ 0x80808080u;
-            const uint32_t lo0 = __byte_perm(w[0], w[1], 0x5140), hi0 = __byte_perm(w[0], w[1], 0x7362);
-            const uint32_t lo1 = __byte_perm(w[2], w[3], 0x5140), hi1 = __byte_perm(w[2], w[3], 0x7362);
+            for (int r = 0; r < 4; ++r) w[r] = *reinterpret_cast<const uint2 *>(vt + place_v<DP>(2 * t + (r & 1) + 8 * (r >> 1), 64 * c + 8 * g));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t sel = (j & 1) ? 0x4342 : 0x4140;
-                const uint32_t b0 = unbias(__byte_perm(j < 2 ? lo0 : hi0, 0x64646464u, sel));
-                const uint32_t b1 = unbias(__byte_perm(j < 2 ? lo1 : hi1, 0x64646464u, sel));
+            for (int q4 = 0; q4 < 2; ++q4) {  // four dims at a time
+                uint32_t x[4];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
+                for (int r = 0; r < 4; ++r) x[r] = (q4 ? w[r].y : w[r].x) ^ 0x80808080u;
+                const uint32_t a0 = __byte_perm(x[0], x[1], 0x5140), a1 = __byte_perm(x[0], x[1], 0x7362);  // dims 0 1, dims 2 3: tokens in pairs
+                const uint32_t b0 = __byte_perm(x[2], x[3], 0x5140), b1 = __byte_perm(x[2], x[3], 0x7362);
 #pragma unroll
-                    for (int q = 0; q < QS; ++q) mma_f16(o[rt][4 * c + j], pf[rt][q], b0, b1);
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t lo = j ? a1 : a0, hi = j ? b1 : b0;
+                    const uint32_t v[4] = {unbias(__byte_perm(lo, 0x64646464u, 0x4140)), unbias(__byte_perm(lo, 0x64646464u, 0x4342)),
+                                           unbias(__byte_perm(hi, 0x64646464u, 0x4140)), unbias(__byte_perm(hi, 0x64646464u, 0x4342))};
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                        for (int q = 0; q < QS; ++q) mma_f16(o[n][4 * c + 2 * q4 + j], v, pf[n][q][0], pf[n][q][1]);
+                }
             }
         }
         __syncwarp();
@@ -461,29 +495,23 @@ template <typename E, int DP, int RT> __global__ void __launch_bounds__(kWarps *
     float *mine_o = reinterpret_cast<float *>(ring);
     float *mine_m = mine_o + L::kRows * DP;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt)
+    for (int n = 0; n < NQ; ++n)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            float l = sum[rt][r];
-            l += __shfl_xor_sync(0xffffffffu, l, 1);
-            l += __shfl_xor_sync(0xffffffffu, l, 2);
-            const float unit = mv[rt][r] == -CUDART_INF_F ? 0.f : exp2_fast(mv[rt][r] - m[rt][r]);
-            const int row = 16 * rt + g + 8 * r;
-            if (t == 0) {
-                mine_m[row] = m[rt][r];
+            float l = sum[n][r];
+#pragma unroll
+            for (int w = 4; w <= 16; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+            const float unit = mv[n][r] == -CUDART_INF_F ? 0.f : exp2_fast(mv[n][r] - m[n][r]);
+            const int row = 8 * n + 2 * t + r;
+            if (g == 0) {
+                mine_m[row] = m[n][r];
                 mine_m[L::kRows + row] = l;
             }
-            // lane t holds dims 8t .. 8t+7 of every 32: four from column 2t, four from column 2t + 1
 #pragma unroll
-            for (int c = 0; c < DP / 32; ++c) {
-                float4 x, y;
-                x.x = o[rt][4 * c][2 * r] * unit, x.y = o[rt][4 * c + 1][2 * r] * unit;
-                x.z = o[rt][4 * c + 2][2 * r] * unit, x.w = o[rt][4 * c + 3][2 * r] * unit;
-                y.x = o[rt][4 * c][2 * r + 1] * unit, y.y = o[rt][4 * c + 1][2 * r + 1] * unit;
-                y.z = o[rt][4 * c + 2][2 * r + 1] * unit, y.w = o[rt][4 * c + 3][2 * r + 1] * unit;
-                float4 *dst = reinterpret_cast<float4 *>(mine_o + row * DP + 32 * c + 8 * t);
-                dst[0] = x;
-                dst[1] = y;
+            for (int c = 0; c < NC; ++c) {
+                float4 *dst = reinterpret_cast<float4 *>(mine_o + row * DP + 64 * c + 8 * g);
+                dst[0] = make_float4(o[n][4 * c][r] * unit, o[n][4 * c][2 + r] * unit, o[n][4 * c + 1][r] * unit, o[n][4 * c + 1][2 + r] * unit);
+                dst[1] = make_float4(o[n][4 * c + 2][r] * unit, o[n][4 * c + 2][2 + r] * unit, o[n][4 * c + 3][r] * unit, o[n][4 * c + 3][2 + r] * unit);
             }
         }
     __syncthreads();
@@ -509,53 +537,47 @@ template <typename E, int DP, int RT> __global__ void __launch_bounds__(kWarps *
         }
         if (a.part) {
             float *dst = a.part + (slot_row * L::kRows + r) * (int64_t)(a.dim + 4);
+            if (r >= live) v = make_float4(0.f, 0.f, 0.f, 0.f), top = -CUDART_INF_F, l = 0.f;  // no query in this row
             *reinterpret_cast<float4 *>(dst + 4 + d) = v;
-            if (d == 0) dst[0] = top, dst[1] = l;
+            if (d == 0) dst[0] = top, dst[1] = l, dst[2] = __int_as_float(count);
             continue;
         }
         const bool dead = r >= live || !(l > 0.f || l != l);
         const float inv = dead ? 0.f : 1.f / l;
         const int token = (row0 + r) / a.group, hq = h * a.group + (row0 + r) % a.group;
         const int64_t at = ((int64_t)s * a.tokens + token) * (a.heads * a.group) + hq;
-        E *dst = static_cast<E *>(a.out) + at * a.dim + d;
-        const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dst[j] = Cvt<float, E>::store(dead ? 0.f : e[j] * inv);
+        store4(static_cast<E *>(a.out) + at * a.dim + d, v, inv, dead);
         if (a.lse && d == 0) a.lse[at] = dead ? -CUDART_INF_F : (top + log2f(l)) * 0.69314718055994531f;
     }
 }
 
-// One warp per output row: joins the pieces of its sequence.
-template <typename E> __global__ void __launch_bounds__(128) k_kv_join(AttnArgs a, int rows_per_block) {
-    const int lane = threadIdx.x & 31;
-    const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);  // row of the output
-    pdl_prologue();
+// One CTA per output row joins the pieces of its sequence: the warps take pieces in turn, lanes the dims.
+constexpr int kJoinWarps = 4;
+template <typename E> __global__ void __launch_bounds__(kJoinWarps * 32) k_kv_join(AttnArgs a, int rows_per_block) {
+    __shared__ float tops[kJoinWarps], sums[kJoinWarps];
+    __shared__ float4 parts[kJoinWarps][64];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t at = blockIdx.x;  // row of the output
     const int64_t all_heads = (int64_t)a.heads * a.group;
-    if (at >= (int64_t)a.seqs * a.tokens * all_heads) return;
     const int hq = (int)(at % all_heads), token = (int)(at / all_heads % a.tokens), s = (int)(at / all_heads / a.tokens);
     const int h = hq / a.group, row = token * a.group + hq % a.group, rb = row / rows_per_block;
-    const int cap = (int)min((long long)a.table_width * a.page, 0x7fffffffll);
-    const int ctx = min(max(a.context[s], 0), cap);
-    const int len = a.qlens ? min(max(a.qlens[s], 0), a.tokens) : a.tokens;
-    const int row0 = rb * rows_per_block;
-    const int live = min(max(len * a.group - row0, 0), rows_per_block);
-    int pieces = 0;
-    if (row - row0 < live) {
-        const Span sp = span_of(a, ctx, len, row0 / a.group, (row0 + live - 1) / a.group);
-        const int n = piece_tokens(a, lane);
-        pieces = sp.hi > sp.lo ? (int)((sp.hi - (sp.lo & ~(kTokens - 1)) + (long long)n - 1) / n) : 0;
-    }
-    const float *part = a.part + (((((int64_t)s * a.heads + h) * a.row_blocks + rb) * a.pieces) * rows_per_block + (row - row0)) * (int64_t)(a.dim + 4);
+    const float *part = a.part + (((((int64_t)s * a.heads + h) * a.row_blocks + rb) * a.pieces) * rows_per_block + (row - rb * rows_per_block)) * (int64_t)(a.dim + 4);
     const int64_t step = (int64_t)rows_per_block * (a.dim + 4);
+    pdl_prologue();
+    const int pieces = __float_as_int(part[2]);  // left there by the first piece
     float top = -CUDART_INF_F;
-    for (int p = lane; p < pieces; p += 32) top = fmaxf(top, part[p * step]);
+    for (int p = threadIdx.x; p < pieces; p += kJoinWarps * 32) top = fmaxf(top, part[p * step]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, tops[w]);
     const float ref = top == -CUDART_INF_F ? 0.f : top;
     float l = 0.f;
     float4 v[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll 4
-    for (int p = 0; p < pieces; ++p) {
+    for (int p = warp; p < pieces; p += kJoinWarps) {
         const float *b = part + p * step;
         const float f = exp2_fast(b[0] - ref);
         l += b[1] * f;
@@ -568,38 +590,47 @@ template <typename E> __global__ void __launch_bounds__(128) k_kv_join(AttnArgs 
             }
         }
     }
+    if (lane == 0) sums[warp] = l;
+    parts[warp][lane] = v[0];
+    parts[warp][32 + lane] = v[1];
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) l += sums[w];
     const bool dead = !(l > 0.f || l != l);
     const float inv = dead ? 0.f : 1.f / l;
+    const int d = 4 * threadIdx.x;
+    if (d < a.dim) {
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-        const int d = 128 * c + 4 * lane;
-        if (d >= a.dim) continue;
-        E *dst = static_cast<E *>(a.out) + at * a.dim + d;
-        const float e[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) dst[j] = Cvt<float, E>::store(dead ? 0.f : e[j] * inv);
+        for (int w = 0; w < kJoinWarps; ++w) {
+            const float4 y = parts[w][threadIdx.x];
+            x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+        }
+        store4(static_cast<E *>(a.out) + at * a.dim + d, x, inv, dead);
     }
-    if (a.lse && lane == 0) a.lse[at] = dead ? -CUDART_INF_F : (top + log2f(l)) * 0.69314718055994531f;
+    if (a.lse && threadIdx.x == 0) a.lse[at] = dead ? -CUDART_INF_F : (top + log2f(l)) * 0.69314718055994531f;
 }
 
-// how a call is cut: row blocks of 16 or 32 rows, pieces along the cache
+// how a call is cut: row blocks of 8, 16 or 32 rows, pieces along the cache
 struct Cut {
-    int row_tiles, row_blocks, pieces, target;
+    int eights, row_blocks, pieces, target;
 };
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens, int64_t table_width, int io_dtype) {
     Cut c;
     const int64_t rows = tokens * group;
-    // two row tiles per warp read and convert the cache once for 32 rows; O and Q of a second tile do not
-    // fit the registers for wider heads, nor for float32's two terms
-    c.row_tiles = rows > 16 && padded_dim(dim) <= 128 && io_dtype != AB_F32 ? 2 : 1;
-    c.row_blocks = (int)std::min<int64_t>(div_up(rows, 16 * c.row_tiles), 1 << 20);
+    // more rows per CTA share the converted codes; O and Q of 32 rows do not fit the registers for wider heads,
+    // nor for float32's two terms
+    c.eights = rows <= 8 ? 1 : rows <= 16 || padded_dim(dim) > 128 || io_dtype == AB_F32 ? 2 : 4;
+    c.row_blocks = (int)std::min<int64_t>(div_up(rows, 8 * c.eights), 1 << 20);
     const int64_t length = table_width * page;
-    const int resident = padded_dim(dim) <= 128 && c.row_tiles == 1 ? 3 : 1;
-    const int64_t slots = (int64_t)sm_count() * resident;
-    c.target = (int)std::max<int64_t>(1, slots / std::max<int64_t>(1, (int64_t)heads * c.row_blocks));
-    const int64_t even = div_up(slots, std::max<int64_t>(1, seqs * heads * c.row_blocks));
-    c.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(div_up(length, kMinPiece), even == 1 ? 2 : 4 * even));
+    const int resident = padded_dim(dim) <= 128 && c.eights <= 2 ? 3 : 1;
+    const int64_t slots = (int64_t)sm_count() * resident, base = std::max<int64_t>(1, seqs * heads * c.row_blocks);
+    const int64_t want = slots * (base >= slots / 2 ? kWaves : 1);
+    c.target = (int)std::max<int64_t>(1, want / std::max<int64_t>(1, (int64_t)heads * c.row_blocks));
+    // a sequence may be cut four times finer than evenly long ones would be
+    c.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(div_up(length, kMinPiece), 4 * div_up(want, base)));
     return c;
 }
 
@@ -612,34 +643,38 @@ int check_call(const ab_kv_cache *c, int64_t seqs, int64_t tokens, int64_t group
         return fail(AB_ERR_UNSUPPORTED, "head_dim=%d: a multiple of 16 up to 256", c->head_dim);
     if (io_dtype != AB_F32 && io_dtype != AB_F16 && io_dtype != AB_BF16) return fail(AB_ERR_UNSUPPORTED, "io_dtype %d", io_dtype);
     if (seqs < 0 || tokens < 0 || group < 1 || table_width < 0 || seqs > 65535 || tokens > (1 << 20) || group > 1024 ||
-        table_width * c->page_size > 0x7fffffffll - 4096)
+        table_width * c->page_size > (1ll << 30))
         return fail(AB_ERR_INVALID, "seqs=%lld tokens=%lld group=%lld table_width=%lld", (long long)seqs, (long long)tokens, (long long)group,
                     (long long)table_width);
     if (c->num_heads < 1 || c->num_heads > 1024) return fail(AB_ERR_INVALID, "num_heads=%d", c->num_heads);
-    if ((int64_t)c->num_heads * div_up(tokens * group, 16) > 65535)
+    if (seqs * tokens * group * c->num_heads > 0x7fffffff || (int64_t)c->num_heads * div_up(tokens * group, 16) > 65535)
         return fail(AB_ERR_UNSUPPORTED, "%lld query rows of %d heads in one call", (long long)(tokens * group), c->num_heads);
     return AB_OK;
 }
 
-template <typename E, int DP, int RT> int launch(const AttnArgs &a, cudaStream_t st) {
-    using L = Layout<E, DP, RT>;
-    const int rc = opt_in_smem<k_kv_attention<E, DP, RT>>(L::kSmem);
+template <typename E, int DP, int NQ, bool FULL> int launch_as(const AttnArgs &a, cudaStream_t st) {
+    using L = Layout<E, DP, NQ>;
+    const int rc = opt_in_smem<k_kv_attention<E, DP, NQ, FULL>>(L::kSmem);
     if (rc != AB_OK) return rc;
-    AB_CUDA_OK(launch_pdl(k_kv_attention<E, DP, RT>, dim3((unsigned)a.pieces, (unsigned)(a.heads * a.row_blocks), (unsigned)a.seqs),
+    AB_CUDA_OK(launch_pdl(k_kv_attention<E, DP, NQ, FULL>, dim3((unsigned)a.pieces, (unsigned)(a.heads * a.row_blocks), (unsigned)a.seqs),
                           dim3(kWarps * 32), L::kSmem, st, a));
     AB_LAUNCH_OK();
-    if (a.part) {
+    if (a.part) {  // (check_call bounds the rows)
         const int64_t rows = (int64_t)a.seqs * a.tokens * a.heads * a.group;
-        AB_CUDA_OK(launch_pdl(k_kv_join<E>, dim3((unsigned)div_up(rows, 4)), dim3(128), 0, st, a, L::kRows));
+        AB_CUDA_OK(launch_pdl(k_kv_join<E>, dim3((unsigned)rows), dim3(kJoinWarps * 32), 0, st, a, L::kRows));
         AB_LAUNCH_OK();
     }
     return AB_OK;
 }
-template <typename E> int dispatch(const AttnArgs &a, int row_tiles, cudaStream_t st) {
+template <typename E, int DP, int NQ> int launch(const AttnArgs &a, cudaStream_t st) {
+    return a.dim == DP ? launch_as<E, DP, NQ, true>(a, st) : launch_as<E, DP, NQ, false>(a, st);
+}
+template <typename E> int dispatch(const AttnArgs &a, int eights, cudaStream_t st) {
     const int dp = padded_dim(a.dim);
     if constexpr (sizeof(E) == 2) {
-        if (row_tiles == 2) return dp == 64 ? launch<E, 64, 2>(a, st) : launch<E, 128, 2>(a, st);
+        if (eights == 4) return dp == 64 ? launch<E, 64, 4>(a, st) : launch<E, 128, 4>(a, st);
     }
+    if (eights == 2) return dp == 64 ? launch<E, 64, 2>(a, st) : dp == 128 ? launch<E, 128, 2>(a, st) : launch<E, 256, 2>(a, st);
     return dp == 64 ? launch<E, 64, 1>(a, st) : dp == 128 ? launch<E, 128, 1>(a, st) : launch<E, 256, 1>(a, st);
 }
 
@@ -655,7 +690,7 @@ extern "C" int64_t aimet_b200_kv_attention_scratch_bytes(const ab_kv_cache *cach
     if (seqs == 0 || tokens == 0) return 0;
     const Cut c = cut_of(cache->num_heads, cache->head_dim, (int)group, cache->page_size, seqs, tokens, table_width, io_dtype);
     if (c.pieces == 1) return 0;
-    return seqs * cache->num_heads * c.row_blocks * c.pieces * 16 * c.row_tiles * (int64_t)(cache->head_dim + 4) * 4;
+    return seqs * cache->num_heads * c.row_blocks * c.pieces * 8 * c.eights * (int64_t)(cache->head_dim + 4) * 4;
 }
 
 extern "C" int aimet_b200_kv_attention(const ab_kv_cache *cache, const void *query, const int64_t *query_strides, void *out, float *lse,
@@ -670,6 +705,7 @@ extern "C" int aimet_b200_kv_attention(const ab_kv_cache *cache, const void *que
     if (!aligned16(cache->key) || !aligned16(cache->value)) return fail(AB_ERR_INVALID, "the cache's codes must be 16-byte aligned");
     if (!query || !query_strides || !out || !context_lens || (table_width > 0 && !block_table)) return fail(AB_ERR_INVALID, "a pointer is NULL");
     if (window < 0 || window > 0x7fffffff) return fail(AB_ERR_INVALID, "window=%lld", (long long)window);
+    if (!aligned16(out)) return fail(AB_ERR_INVALID, "out must be 16-byte aligned");
     if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
         return fail(AB_ERR_SCRATCH, "scratch of %lld bytes, 16-byte aligned, is needed (got %lld)", (long long)need, (long long)scratch_bytes);
     const Cut cut = cut_of(cache->num_heads, cache->head_dim, (int)group, cache->page_size, seqs, tokens, table_width, io_dtype);
@@ -695,6 +731,8 @@ extern "C" int aimet_b200_kv_attention(const ab_kv_cache *cache, const void *que
     a.context = context_lens;
     a.qlens = query_lens;
     a.table_stride = table_stride;
+    const int per_page = cache->page_size / kTokens;
+    a.page_magic = per_page == 1 ? 0 : (uint32_t)(((1ull << 32) + per_page - 1) / per_page);
     a.table_width = (int)table_width;
     a.seqs = (int)seqs;
     a.tokens = (int)tokens;
@@ -707,8 +745,8 @@ extern "C" int aimet_b200_kv_attention(const ab_kv_cache *cache, const void *que
     a.scale_log2 = (float)(softmax_scale * 1.4426950408889634);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (io_dtype) {
-        case AB_F32: return dispatch<float>(a, cut.row_tiles, st);
-        case AB_F16: return dispatch<__half>(a, cut.row_tiles, st);
-        default: return dispatch<__nv_bfloat16>(a, cut.row_tiles, st);
+        case AB_F32: return dispatch<float>(a, cut.eights, st);
+        case AB_F16: return dispatch<__half>(a, cut.eights, st);
+        default: return dispatch<__nv_bfloat16>(a, cut.eights, st);
     }
 }
