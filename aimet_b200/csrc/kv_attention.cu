@@ -625,7 +625,9 @@ Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens
     c.eights = rows <= 8 ? 1 : rows <= 16 || padded_dim(dim) > 128 || io_dtype == AB_F32 ? 2 : 4;
     c.row_blocks = (int)std::min<int64_t>(div_up(rows, 8 * c.eights), 1 << 20);
     const int64_t length = table_width * page;
-    const int resident = padded_dim(dim) <= 128 && c.eights <= 2 ? 3 : 1;
+    // CTAs on an SM, by registers and shared memory
+    const int wide = padded_dim(dim);
+    const int resident = wide == 256 ? 1 : c.eights == 1 ? (wide == 64 ? 5 : 3) : c.eights == 2 && wide == 64 ? 4 : 2;
     const int64_t slots = (int64_t)sm_count() * resident, base = std::max<int64_t>(1, seqs * heads * c.row_blocks);
     const int64_t want = slots * (base >= slots / 2 ? kWaves : 1);
     c.target = (int)std::max<int64_t>(1, want / std::max<int64_t>(1, (int64_t)heads * c.row_blocks));

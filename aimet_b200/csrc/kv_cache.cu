@@ -51,33 +51,71 @@ struct AppendArgs {
     int vec[2];
 };
 
-struct Quantizer {
-    float s, r, lim;
-    bool plain;
-    __device__ __forceinline__ explicit Quantizer(float scale) {
-        s = scale;
-        plain = !(scale >= 7.8886090522101181e-31f && scale <= 1.2676506002282294e30f);  // 2^-100, 2^100
-        r = plain ? 0.f : __frcp_rn(scale);
-        lim = __fmul_rn(scale, kLevels);
+// The largest magnitude of a piece as the bits of its type (whose order is that of the magnitudes; infinities
+// and NaN are the largest), two 16-bit elements at a time.
+__device__ __forceinline__ uint32_t max_bits(const Vec16<float> &v, uint32_t top) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(v.v[e]) & 0x7fffffffu);
+    return top;
+}
+template <typename E> __device__ __forceinline__ uint32_t max_bits(const Vec16<E> &v, uint32_t top) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = __vmaxu2(top, w[e] & 0x7fff7fffu);
+    return top;
+}
+__device__ __forceinline__ uint32_t fold_bits(uint32_t top, float) { return top; }
+template <typename E> __device__ __forceinline__ uint32_t fold_bits(uint32_t top, E) { return max(top & 0xffffu, top >> 16); }
+__device__ __forceinline__ float value_of(uint32_t bits, float) { return __uint_as_float(bits); }
+__device__ __forceinline__ float value_of(uint32_t bits, __nv_bfloat16) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ float value_of(uint32_t bits, __half) { return __half2float(__ushort_as_half((unsigned short)bits)); }
+
+constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it rounds half to even into the low bits
+
+// The code of a finite x, |x| <= scale * 127 (1 + 2^-22) and scale in [2^-100, 2^100], in the low byte (two's
+// complement): the correctly rounded quotient without the divide unit.
+__device__ __forceinline__ uint32_t code_fast(float x, float s, float r) {
+    const float q0 = __fmul_rn(x, r);
+    return __float_as_uint(__fadd_rn(__fmaf_rn(__fmaf_rn(-q0, s, x), r, q0), kRound));
+}
+// Any x and scale: NaN gives 0, infinities the outermost levels, a zero scale zeros.
+__device__ __forceinline__ uint32_t code_any(float x, float s) {
+    x = x == x ? x : 0.f;
+    const float q = s > 0.f ? __fdiv_rn(x, s) : 0.f;
+    return __float_as_uint(__fadd_rn(fminf(fmaxf(q, -kLevels), kLevels), kRound));
+}
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// the largest of the CTA's values, for every thread
+template <int THREADS> __device__ __forceinline__ uint32_t block_max(uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
+    if (THREADS > 32) {
+        __shared__ uint32_t of_warp[THREADS / 32];
+        __syncthreads();  // a second use may follow the first at once
+        if ((threadIdx.x & 31) == 0) of_warp[threadIdx.x >> 5] = v;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) v = max(v, of_warp[w]);
     }
-    // the code in the low byte (two's complement); NaN gives 0, infinities the outermost levels
-    __device__ __forceinline__ uint32_t operator()(float x) const {
-        x = x == x ? x : 0.f;
-        float q;
-        if (plain) {
-            q = s > 0.f ? __fdiv_rn(x, s) : 0.f;
-        } else {
-            x = fminf(fmaxf(x, -lim), lim);
-            const float q0 = __fmul_rn(x, r);
-            q = __fmaf_rn(__fmaf_rn(-q0, s, x), r, q0);
-        }
-        q = fminf(fmaxf(q, -kLevels), kLevels);
-        return __float_as_uint(__fadd_rn(q, 12582912.f)) & 0xffu;  // 1.5 * 2^23: rounds half to even
+    return v;
+}
+
+// Walks the 16-byte pieces (per_row of them in a row) of a block, THREADS apart, without a division per piece.
+struct Piece {
+    int row, piece;
+    __device__ __forceinline__ Piece(int first, int per_row) : row(first / per_row), piece(first % per_row) {}
+    __device__ __forceinline__ void advance(int rows, int pieces, int per_row) {
+        row += rows;
+        piece += pieces;
+        if (piece >= per_row) piece -= per_row, ++row;
     }
 };
 
-template <typename E, int THREADS> __global__ void __launch_bounds__(THREADS) k_kv_append(AppendArgs a) {
-    constexpr int V = 16 / sizeof(E);  // elements per 16-byte vector
+// KEEP pieces of a thread stay in registers between the two passes; a block with more is read again (from L1 or L2).
+template <typename E, int THREADS, int KEEP> __global__ void __launch_bounds__(THREADS) k_kv_append(AppendArgs a) {
+    constexpr int V = 16 / sizeof(E);  // elements per 16-byte piece
     pdl_prologue();
     int64_t at = blockIdx.x;
     const int kv = (int)(at & 1);
@@ -92,49 +130,63 @@ template <typename E, int THREADS> __global__ void __launch_bounds__(THREADS) k_
     const int64_t lo = max(b * page, ctx), hi = min((b + 1) * page, ctx + len);  // positions of its new tokens
     if (lo >= hi || b >= a.table_width) return;
     const int64_t pg = a.table[(int64_t)s * a.table_stride + b];
-    if (pg < 0 || pg >= a.c.pages) return;
 
     const int kept = (int)(lo - b * page), rows = (int)(hi - lo);
-    const E *x = static_cast<const E *>(a.x[kv]) + (int64_t)s * a.stride_s[kv] + (int64_t)h * a.stride_h[kv] + (lo - ctx) * a.stride_t[kv];
     const int64_t stride_t = a.stride_t[kv];
+    const E *x = static_cast<const E *>(a.x[kv]) + (int64_t)s * a.stride_s[kv] + (int64_t)h * a.stride_h[kv] + (lo - ctx) * stride_t;
+    const bool vec = a.vec[kv];
+    const int per_row = dim / V, step_rows = THREADS / per_row, step_pieces = THREADS % per_row;
+    auto load = [&](const Piece &p) {
+        const E *src = x + p.row * stride_t + p.piece * V;
+        Vec16<E> v;
+        if (vec) {
+            v = *reinterpret_cast<const Vec16<E> *>(src);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) v.v[e] = src[e];
+        }
+        return v;
+    };
+
+    // the new tokens are requested before the page is known
+    Vec16<E> keep[KEEP];
+    uint32_t bits = 0;
+    Piece p(threadIdx.x, per_row);
+    const Piece first = p;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        if (p.row < rows) keep[i] = load(p);
+        p.advance(step_rows, step_pieces, per_row);
+    }
+    for (; p.row < rows; p.advance(step_rows, step_pieces, per_row)) bits = max_bits(load(p), bits);
+    p = first;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        if (p.row < rows) bits = max_bits(keep[i], bits);
+        p.advance(step_rows, step_pieces, per_row);
+    }
+    bits = fold_bits(bits, E());
+    if (pg < 0 || pg >= a.c.pages) return;  // (the CTA's threads agree)
     int8_t *code = a.c.code[kv] + ((pg * a.c.heads + h) * page) * (int64_t)dim;
     float *scale_at = a.c.scale[kv] + pg * a.c.heads + h;
-    const bool vec = a.vec[kv];
-    const int per_row = dim / V, work = rows * per_row;
-
-    float top = 0.f;
-    for (int i = threadIdx.x; i < work; i += THREADS) {
-        const int r = i / per_row, d = (i - r * per_row) * V;
-        const E *p = x + r * stride_t + d;
-        Vec16<E> v;
-        if (vec)
-            v = *reinterpret_cast<const Vec16<E> *>(p);
-        else
-#pragma unroll
-            for (int e = 0; e < V; ++e) v.v[e] = p[e];
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float m = fabsf(to_f32(v.v[e]));
-            top = fmaxf(top, m <= 3.402823466e38f ? m : 0.f);  // finite values only
-        }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (THREADS > 32) {
-        __shared__ float tops[THREADS / 32];
-        if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
-    }
-
     const float old = kept ? *scale_at : 0.f;
+    bits = block_max<THREADS>(bits);  // (everyone has read the old scale)
+    float top = value_of(bits, E());
+    const bool finite = top <= 3.402823466e38f;
+    if (!finite) {  // the largest of the finite values
+        top = 0.f;
+        for (p = first; p.row < rows; p.advance(step_rows, step_pieces, per_row)) {
+            const Vec16<E> v = load(p);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float m = fabsf(to_f32(v.v[e]));
+                top = fmaxf(top, m <= 3.402823466e38f ? m : 0.f);
+            }
+        }
+        top = __uint_as_float(block_max<THREADS>(__float_as_uint(top)));
+    }
     float scale = __fmul_rn(top, 1.f / kLevels);
     if (kept) scale = scale <= old ? old : fmaxf(scale, __fmul_rn(old, kGrowth));
-    if (THREADS > 32)
-        __syncthreads();  // everyone has read the old scale
-    else
-        __syncwarp();
     if (threadIdx.x == 0) *scale_at = scale;
 
     if (kept && scale != old) {  // the codes held so far move onto the coarser grid
@@ -146,35 +198,42 @@ template <typename E, int THREADS> __global__ void __launch_bounds__(THREADS) k_
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float q = __fmul_rn((float)(int8_t)(v >> (8 * e)), ratio);
-                o |= (__float_as_uint(__fadd_rn(q, 12582912.f)) & 0xffu) << (8 * e);
+                o |= (__float_as_uint(__fadd_rn(q, kRound)) & 0xffu) << (8 * e);
             }
             w[i] = o;
         }
     }
 
-    const Quantizer q(scale);
+    const bool fast = finite && scale >= 7.8886090522101181e-31f && scale <= 1.2676506002282294e30f;  // 2^-100, 2^100
+    const float r = fast ? __frcp_rn(scale) : 0.f;
     int8_t *out = code + (int64_t)kept * dim;
-    for (int i = threadIdx.x; i < work; i += THREADS) {
-        const int r = i / per_row, d = (i - r * per_row) * V;
-        const E *p = x + r * stride_t + d;
-        Vec16<E> v;
-        if (vec)
-            v = *reinterpret_cast<const Vec16<E> *>(p);
-        else
-#pragma unroll
-            for (int e = 0; e < V; ++e) v.v[e] = p[e];
+    auto store = [&](const Piece &p, const Vec16<E> &v) {
         uint32_t o[V / 4];
 #pragma unroll
         for (int e = 0; e < V / 4; ++e) {
-            o[e] = q(to_f32(v.v[4 * e])) | q(to_f32(v.v[4 * e + 1])) << 8 | q(to_f32(v.v[4 * e + 2])) << 16 |
-                   q(to_f32(v.v[4 * e + 3])) << 24;
+            uint32_t c[4];
+            if (fast) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[j] = code_fast(to_f32(v.v[4 * e + j]), scale, r);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) c[j] = code_any(to_f32(v.v[4 * e + j]), scale);
+            }
+            o[e] = low_bytes(c[0], c[1], c[2], c[3]);
         }
-        int8_t *dst = out + (int64_t)r * dim + d;
+        int8_t *dst = out + p.row * dim + p.piece * V;
         if constexpr (V == 8)
             *reinterpret_cast<uint2 *>(dst) = make_uint2(o[0], o[1]);
         else
             *reinterpret_cast<uint32_t *>(dst) = o[0];
+    };
+    p = first;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        if (p.row < rows) store(p, keep[i]);
+        p.advance(step_rows, step_pieces, per_row);
     }
+    for (; p.row < rows; p.advance(step_rows, step_pieces, per_row)) store(p, load(p));
 }
 
 // ---------------------------------------------------------------------------------------------------
@@ -207,22 +266,42 @@ template <typename E> __global__ void __launch_bounds__(128) k_kv_gather(GatherA
     const float scale = there ? a.c.scale[kv][pg * a.c.heads + h] : 0.f;
     E *y = static_cast<E *>(a.y[kv]) + (((int64_t)s * a.length + first) * a.c.heads + h) * dim;
     const int64_t pitch = (int64_t)a.c.heads * dim;
-    const int per_row = dim / 16;
-    for (int i = threadIdx.x; i < rows * per_row; i += 128) {
-        const int r = i / per_row, d = (i - r * per_row) * 16;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < there) v = *reinterpret_cast<const uint4 *>(code + (int64_t)r * dim + d);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        constexpr int V = 16 / sizeof(E);
-        Vec16<E> o[16 / V];
+    // kAhead pieces of a thread requested before the first is stored
+    constexpr int V = 16 / sizeof(E), kAhead = 4;
+    const int per_row = dim / 16, step_rows = 128 / per_row, step_pieces = 128 % per_row;
+    Piece p(threadIdx.x, per_row);
+    while (p.row < rows) {
+        const Piece first = p;
+        uint4 v[kAhead];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float f = r < there ? __fmul_rn((float)(int8_t)(w[e / 4] >> (8 * (e % 4))), scale) : 0.f;
-            o[e / V].v[e % V] = Cvt<float, E>::store(f);
+        for (int i = 0; i < kAhead; ++i) {
+            v[i] = make_uint4(0, 0, 0, 0);
+            if (p.row < there) v[i] = *reinterpret_cast<const uint4 *>(code + (int64_t)p.row * dim + p.piece * 16);
+            p.advance(step_rows, step_pieces, per_row);
         }
-        Vec16<E> *dst = reinterpret_cast<Vec16<E> *>(y + r * pitch + d);
+        p = first;
 #pragma unroll
-        for (int e = 0; e < 16 / V; ++e) dst[e] = o[e];
+        for (int i = 0; i < kAhead; ++i) {
+            if (p.row < rows) {
+                // code + 128 in the mantissa of 2^23, minus 2^23 + 128: the conversion pipe is the slower way
+                const uint32_t w[4] = {v[i].x ^ 0x80808080u, v[i].y ^ 0x80808080u, v[i].z ^ 0x80808080u, v[i].w ^ 0x80808080u};
+                const float f = p.row < there ? scale : 0.f;
+                Vec16<E> *dst = reinterpret_cast<Vec16<E> *>(y + p.row * pitch + p.piece * 16);
+#pragma unroll
+                for (int e = 0; e < 16 / V; ++e) {
+                    float q[V];
+                    Vec16<E> o;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) {
+                        const int c = e * V + j;
+                        q[j] = __fmul_rn(__uint_as_float(__byte_perm(w[c / 4], 0x4b000000u, 0x7650 + c % 4)) - 8388736.f, f);
+                    }
+                    VecCvt<float, E>::pack(q, o);
+                    dst[e] = o;
+                }
+            }
+            p.advance(step_rows, step_pieces, per_row);
+        }
     }
 }
 
@@ -247,16 +326,17 @@ int check_cache(const ab_kv_cache *c, CacheView *v) {
     return AB_OK;
 }
 
-template <typename E, int THREADS> int launch_append(const AppendArgs &a, int64_t ctas, cudaStream_t st) {
-    AB_CUDA_OK(launch_pdl(k_kv_append<E, THREADS>, dim3((unsigned)ctas), dim3(THREADS), 0, st, a));
+template <typename E, int THREADS, int KEEP> int launch_append(const AppendArgs &a, int64_t ctas, cudaStream_t st) {
+    AB_CUDA_OK(launch_pdl(k_kv_append<E, THREADS, KEEP>, dim3((unsigned)ctas), dim3(THREADS), 0, st, a));
     AB_LAUNCH_OK();
     return AB_OK;
 }
 template <typename E> int dispatch_append(const AppendArgs &a, int64_t ctas, cudaStream_t st) {
-    // a warp is enough for a few rows and leaves no barriers; whole blocks take 256 threads
-    const int rows = std::min(a.tokens, a.c.page);
-    if ((int64_t)rows * a.c.dim <= 1024) return launch_append<E, 32>(a, ctas, st);
-    return launch_append<E, 256>(a, ctas, st);
+    // a warp is enough for a few rows and leaves no barriers; whole blocks take as many threads as hold them in registers
+    const int64_t pieces = (int64_t)std::min(a.tokens, a.c.page) * a.c.dim * sizeof(E) / 16;
+    if (pieces <= 128) return launch_append<E, 32, 4>(a, ctas, st);
+    if (pieces <= 512) return launch_append<E, 128, 4>(a, ctas, st);
+    return launch_append<E, 256, 8>(a, ctas, st);
 }
 
 }  // namespace
