@@ -82,6 +82,11 @@ __device__ __forceinline__ void pdl_prologue() {
     pdl_wait();
 }
 
+// all threads of a cluster's CTAs; what was written to shared memory before is visible to all after
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                               Args &&...args) {

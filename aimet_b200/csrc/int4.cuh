@@ -107,10 +107,6 @@ template <> struct Packed<int8_t, 1> { using V = int8_t; static __device__ __for
 template <> struct Packed<int8_t, 2> { using V = uint16_t; static __device__ __forceinline__ float get(V v, int i) { return (float)(int8_t)(v >> (8 * i)); } };
 template <> struct Packed<int8_t, 4> { using V = uint32_t; static __device__ __forceinline__ float get(V v, int i) { return (float)(int8_t)(v >> (8 * i)); } };
 
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
 // y for many tokens (int4_gemm.cu): 16-bit x, 16-byte aligned rows.  block, mult: as in the descriptor.
 struct Int4Gemm {
     Int4View w;

@@ -48,6 +48,7 @@ constexpr int kMinPiece = 128, kMaxMinPiece = 512;
 // Pieces per CTA slot of the machine: one where pieces are all that fills it (two of 131072 tokens: 108 us, 119 with
 // two); three where sequences and heads do, so that ragged lengths even out (64 of 1000 to 4000: 99 us, 106 with one).
 constexpr int kWaves = 3;
+constexpr int kMostCluster = 8, kClusterPiece = 1024;
 
 struct AttnArgs {
     const int8_t *key, *value;
@@ -147,6 +148,22 @@ template <typename E> __device__ __forceinline__ void load_row16(const E *p, int
     }
 }
 
+__device__ __forceinline__ uint32_t in_cluster(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 // four neighbouring results, scaled (dims are multiples of 16 and outputs 16-byte aligned)
 template <typename E> __device__ __forceinline__ void store4(E *dst, const float4 &v, float inv, bool dead) {
     const float e[4] = {dead ? 0.f : v.x * inv, dead ? 0.f : v.y * inv, dead ? 0.f : v.z * inv, dead ? 0.f : v.w * inv};
@@ -205,7 +222,7 @@ template <typename E, int DP, int NQ> struct Layout {
     static constexpr int kRows = 8 * NQ;                     // query rows of a CTA
     static constexpr int kJoin = kRows * DP * 4 + kRows * 8;  // a warp's O, maxima and sums
     static constexpr int kPerWarp = kWarp > kJoin ? kWarp : (kJoin + 127) / 128 * 128;
-    static constexpr int kSmem = kWarps * kPerWarp;
+    static constexpr int kSmem = kWarps * kPerWarp + kJoin;  // and a cluster's part
 };
 
 // FULL: the head's dim is DP, a constant
@@ -238,6 +255,12 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
         to = (int)min((long long)to, p0 + n);
         if (piece > 0 && from >= to) return;
         count = max(1, (span.hi - start + n - 1) / n);
+    } else if (a.pieces > 1) {  // a cluster: even parts of this sequence
+        const int start = span.lo & ~(kTokens - 1);
+        const int n = max(((to - start + a.pieces - 1) / a.pieces + 63) / 64 * 64, kMinPiece);
+        const long long p0 = (long long)start + (long long)piece * n;
+        from = (int)min((long long)to, max((long long)from, p0));
+        to = (int)min((long long)to, p0 + n);
     }
 
     const int tile0 = from / kTokens, tiles = from < to ? (to - 1) / kTokens - tile0 + 1 : 0;
@@ -519,6 +542,15 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
     const int stored = min(L::kRows, rows - row0);  // rows of the output in this block
     const int per_row = a.dim / 4;
     const int64_t slot_row = (((int64_t)s * a.heads + h) * a.row_blocks + rb) * a.pieces + piece;
+    auto emit = [&](int r, int d, const float4 &v, float top, float l) {
+        const bool dead = r >= live || !(l > 0.f || l != l);
+        const float inv = dead ? 0.f : 1.f / l;
+        const int token = (row0 + r) / a.group, hq = h * a.group + (row0 + r) % a.group;
+        const int64_t at = ((int64_t)s * a.tokens + token) * (a.heads * a.group) + hq;
+        store4(static_cast<E *>(a.out) + at * a.dim + d, v, inv, dead);
+        if (a.lse && d == 0) a.lse[at] = dead ? -CUDART_INF_F : (top + log2f(l)) * 0.69314718055994531f;
+    };
+    float *joined = reinterpret_cast<float *>(smem + kWarps * L::kPerWarp);  // of a cluster's CTA: O, maxima, sums
     for (int i = threadIdx.x; i < stored * per_row; i += kWarps * 32) {
         const int r = i / per_row, d = (i - r * per_row) * 4;
         float top = -CUDART_INF_F;
@@ -540,15 +572,34 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
             if (r >= live) v = make_float4(0.f, 0.f, 0.f, 0.f), top = -CUDART_INF_F, l = 0.f;  // no query in this row
             *reinterpret_cast<float4 *>(dst + 4 + d) = v;
             if (d == 0) dst[0] = top, dst[1] = l, dst[2] = __int_as_float(count);
-            continue;
+        } else if (a.pieces > 1) {
+            *reinterpret_cast<float4 *>(joined + r * DP + d) = v;
+            if (d == 0) joined[L::kRows * DP + r] = top, joined[L::kRows * DP + L::kRows + r] = l;
+        } else {
+            emit(r, d, v, top, l);
         }
-        const bool dead = r >= live || !(l > 0.f || l != l);
-        const float inv = dead ? 0.f : 1.f / l;
-        const int token = (row0 + r) / a.group, hq = h * a.group + (row0 + r) % a.group;
-        const int64_t at = ((int64_t)s * a.tokens + token) * (a.heads * a.group) + hq;
-        store4(static_cast<E *>(a.out) + at * a.dim + d, v, inv, dead);
-        if (a.lse && d == 0) a.lse[at] = dead ? -CUDART_INF_F : (top + log2f(l)) * 0.69314718055994531f;
     }
+    if (a.part || a.pieces == 1) return;
+    // join the cluster's CTAs through distributed shared memory, every CTA a share of the output
+    cluster_barrier();
+    const uint32_t base = smem_u32(joined);
+    for (int i = piece * (kWarps * 32) + threadIdx.x; i < stored * per_row; i += a.pieces * (kWarps * 32)) {
+        const int r = i / per_row, d = (i - r * per_row) * 4;
+        float top = -CUDART_INF_F, l = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < a.pieces; ++c) {
+            const uint32_t there = in_cluster(base, c);
+            const float mc = ld_cluster(there + (L::kRows * DP + r) * 4), lc = ld_cluster(there + (L::kRows * DP + L::kRows + r) * 4);
+            const float4 x = ld_cluster4(there + (r * DP + d) * 4);
+            const float next_top = fmaxf(top, mc), ref = next_top == -CUDART_INF_F ? 0.f : next_top;
+            const float f = exp2_fast(top - ref), g2 = exp2_fast(mc - ref);
+            l = l * f + lc * g2;
+            v.x = v.x * f + x.x * g2, v.y = v.y * f + x.y * g2, v.z = v.z * f + x.z * g2, v.w = v.w * f + x.w * g2;
+            top = next_top;
+        }
+        emit(r, d, v, top, l);
+    }
+    cluster_barrier();  // nobody leaves while its part is being read
 }
 
 // One CTA per output row joins the pieces of its sequence: the warps take pieces in turn, lanes the dims.
@@ -615,6 +666,7 @@ template <typename E> __global__ void __launch_bounds__(kJoinWarps * 32) k_kv_jo
 // how a call is cut: row blocks of 8, 16 or 32 rows, pieces along the cache
 struct Cut {
     int eights, row_blocks, pieces, target;
+    bool cluster;  // the pieces of a row block are a cluster of CTAs; otherwise they leave partial results in scratch
 };
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens, int64_t table_width, int io_dtype) {
@@ -631,8 +683,12 @@ Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens
     const int64_t slots = (int64_t)sm_count() * resident, base = std::max<int64_t>(1, seqs * heads * c.row_blocks);
     const int64_t want = slots * (base >= slots / 2 ? kWaves : 1);
     c.target = (int)std::max<int64_t>(1, want / std::max<int64_t>(1, (int64_t)heads * c.row_blocks));
-    // a sequence may be cut four times finer than evenly long ones would be
-    c.pieces = (int)std::max<int64_t>(1, std::min<int64_t>(div_up(length, kMinPiece), 4 * div_up(want, base)));
+    // Eight pieces or fewer, or contexts that eight CTAs are not long over, are joined through the cluster's shared
+    // memory (one launch, no scratch): one of 500 tokens CLUSTER_NOTE.
+    const int64_t wanted = div_up(want, base), most = std::max<int64_t>(1, div_up(length, kMinPiece));
+    c.cluster = std::min(wanted, most) <= kMostCluster || length <= kMostCluster * kClusterPiece;
+    // otherwise a sequence may be cut four times finer than evenly long ones would be
+    c.pieces = (int)(c.cluster ? std::min<int64_t>(kMostCluster, std::min(wanted, most)) : std::min(most, 4 * wanted));
     return c;
 }
 
@@ -658,8 +714,20 @@ template <typename E, int DP, int NQ, bool FULL> int launch_as(const AttnArgs &a
     using L = Layout<E, DP, NQ>;
     const int rc = opt_in_smem<k_kv_attention<E, DP, NQ, FULL>>(L::kSmem);
     if (rc != AB_OK) return rc;
-    AB_CUDA_OK(launch_pdl(k_kv_attention<E, DP, NQ, FULL>, dim3((unsigned)a.pieces, (unsigned)(a.heads * a.row_blocks), (unsigned)a.seqs),
-                          dim3(kWarps * 32), L::kSmem, st, a));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.pieces, (unsigned)(a.heads * a.row_blocks), (unsigned)a.seqs);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = L::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = a.pieces;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = !a.part && a.pieces > 1 ? 2 : 1;
+    AB_CUDA_OK(cudaLaunchKernelEx(&cfg, k_kv_attention<E, DP, NQ, FULL>, a));
     AB_LAUNCH_OK();
     if (a.part) {  // (check_call bounds the rows)
         const int64_t rows = (int64_t)a.seqs * a.tokens * a.heads * a.group;
@@ -691,7 +759,7 @@ extern "C" int64_t aimet_b200_kv_attention_scratch_bytes(const ab_kv_cache *cach
     if (rc != AB_OK) return rc;
     if (seqs == 0 || tokens == 0) return 0;
     const Cut c = cut_of(cache->num_heads, cache->head_dim, (int)group, cache->page_size, seqs, tokens, table_width, io_dtype);
-    if (c.pieces == 1) return 0;
+    if (c.cluster) return 0;
     return seqs * cache->num_heads * c.row_blocks * c.pieces * 8 * c.eights * (int64_t)(cache->head_dim + 4) * 4;
 }
 

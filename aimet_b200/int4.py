@@ -22,6 +22,7 @@ from ._lib import check, lib
 __all__ = ["PackedInt4Weight", "linear_int4"]
 
 _TILE_N, _TILE_K, _CHUNK_K = 16, 64, 256
+_MOST_PLANS = 512  # input layouts that a weight remembers
 _MAX_ZERO = 112  # 16-bit floats subtract zero points up to here exactly
 
 
@@ -90,6 +91,9 @@ class PackedInt4Weight:
         self._desc = _lib.Int4Weight(out_features, in_features, storage, int(multiples), zero, 0,
                                      codes.data_ptr(), scales.data_ptr(), _lib.ptr(zeros), row_scale.data_ptr())
         self.device = codes.device
+        self._ref = ctypes.byref(self._desc)
+        _status.pointer(self.device)  # made now: a first product may be inside a stream capture, where it could not be
+        self._plans: dict = {}  # layout of an input -> what follows from it
 
     @property
     def nbytes(self) -> int:
@@ -213,37 +217,60 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
     float32, float16 or bfloat16 activations; sums in float32, one rounding to ``input.dtype``.  For
     inference: an input or bias that needs a gradient is refused (train through the quantizer instead).
     """
-    if not input.is_cuda:
-        raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
-    code = _lib.DTYPE_CODE.get(input.dtype)
-    if code is None or code == _lib.AB_F64:
-        raise NotImplementedError(f"linear_int4 takes float32, float16 or bfloat16 activations, got {input.dtype}")
-    if input.dim() == 0 or input.shape[-1] != weight.in_features:
-        raise RuntimeError(f"expected {weight.in_features} input features, got an input of shape {tuple(input.shape)}")
-    if input.device != weight.device:
-        raise RuntimeError(f"input is on {input.device}, the weight on {weight.device}")
+    signature = (input.shape, input.stride(), input.dtype, input.device)
+    plan = weight._plans.get(signature)  # pylint: disable=protected-access
+    if plan is None:
+        plan = _plan_linear(signature, input, weight)
     if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("linear_int4 has no backward pass: call it under torch.no_grad(), or train through the weight's quantizer")
+    code, tokens, pitch, out_shape, direct, watched = plan
     if bias is not None:
         if bias.dtype != input.dtype or bias.device != input.device or tuple(bias.shape) != (weight.out_features,):
             raise RuntimeError(f"bias must be {input.dtype} of shape {(weight.out_features,)} on {input.device}, "
                                f"got {bias.dtype} of shape {tuple(bias.shape)} on {bias.device}")
         bias = bias.contiguous()
-    out = torch.empty(input.shape[:-1] + (weight.out_features,), dtype=input.dtype, device=input.device)
-    tokens = math.prod(input.shape[:-1])
+    out = input.new_empty(out_shape)
     if tokens == 0:
         return out
-    x = input.reshape(tokens, weight.in_features)
-    size = x.element_size()
-    if x.stride(1) != 1 or (tokens > 1 and x.stride(0) < weight.in_features):  # rows that overlap: an expanded input
-        x = x.contiguous()
-    status = None
-    if tokens > 2 and size == 2:  # the library may choose its tensor-core kernel, which has bounded waits
-        status = _status.pointer(input.device)
-        if tokens > 16 and (x.data_ptr() % 16 or x.stride(0) % 8):  # it tensor-core kernel wants rows that start on 16 bytes
-            padded = x.new_empty(tokens, -(-weight.in_features // 8) * 8)[:, : weight.in_features]
-            x = padded.copy_(x)
-    with _lib.on_device(input.device):
-        check(lib.aimet_b200_int4_linear(weight._desc, x.data_ptr(), x.stride(0), None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
-                                         weight.out_features, tokens, code, status, _lib.stream_ptr(input.device)))
+    if not direct:
+        input = input.reshape(tokens, weight.in_features).contiguous()
+    if tokens > 16 and watched and (input.data_ptr() % 16 or pitch % 8):  # the tensor-core kernel wants rows that start on 16 bytes
+        pitch = -(-weight.in_features // 8) * 8
+        rows = input.reshape(tokens, weight.in_features)
+        input = rows.new_empty(tokens, pitch)[:, : weight.in_features].copy_(rows)
+    status = _status.pointer(weight.device) if watched else None
+    with _lib.on_device(weight.device):
+        check(lib.aimet_b200_int4_linear(weight._ref, input.data_ptr(), pitch, None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
+                                         weight.out_features, tokens, code, status, _lib.stream_ptr(weight.device)))
     return out
+
+
+def _plan_linear(signature, x: torch.Tensor, weight: PackedInt4Weight):
+    """Checks an input and says how it is read: dtype code, tokens, elements between rows, output shape, whether it
+    can be read where it is, whether the library may choose its tensor-core kernel."""
+    if not x.is_cuda:
+        raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
+    code = _lib.DTYPE_CODE.get(x.dtype)
+    if code is None or code == _lib.AB_F64:
+        raise NotImplementedError(f"linear_int4 takes float32, float16 or bfloat16 activations, got {x.dtype}")
+    k = weight.in_features
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise RuntimeError(f"expected {k} input features, got an input of shape {tuple(x.shape)}")
+    if x.device != weight.device:
+        raise RuntimeError(f"input is on {x.device}, the weight on {weight.device}")
+    tokens = math.prod(x.shape[:-1])
+    pitch, direct = k, True
+    if tokens:
+        # rows at one distance from each other, elements side by side, no overlap
+        direct = x.stride(-1) == 1 or k == 1
+        outer = [(n, st) for n, st in zip(x.shape[:-1], x.stride()[:-1]) if n > 1]
+        if outer:
+            pitch = outer[-1][1]
+            direct = direct and pitch >= k and all(a[1] == b[0] * b[1] for a, b in zip(outer, outer[1:]))
+        if not direct:
+            pitch = k
+    plan = (code, tokens, pitch, x.shape[:-1] + (weight.out_features,), direct, tokens > 2 and code != _lib.AB_F32)
+    if len(weight._plans) >= _MOST_PLANS:  # pylint: disable=protected-access
+        weight._plans.clear()  # pylint: disable=protected-access
+    weight._plans[signature] = plan  # pylint: disable=protected-access
+    return plan

@@ -22,10 +22,12 @@ from ._lib import check, lib
 __all__ = ["Int8KVCache"]
 
 _Strides = ctypes.c_int64 * 3
+_MOST_PLANS = 512  # checked argument layouts that a cache remembers
 
 
-def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+def _signature(t: Optional[torch.Tensor]):
+    """What the checks of an argument depend on (nothing of its values or address)."""
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
 
 
 class Int8KVCache:
@@ -85,13 +87,22 @@ class Int8KVCache:
         self.device = key.device
         self._desc = _lib.KVCache(key.data_ptr(), value.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(),
                                   self.num_pages, self.num_heads, self.page_size, self.head_dim, 0)
+        self._ref = ctypes.byref(self._desc)
+        self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
+        self._plans: dict = {}  # signature of a call's arguments -> what follows from it
+
+    def _remember(self, signature, plan):
+        if len(self._plans) >= _MOST_PLANS:
+            self._plans.clear()
+        self._plans[signature] = plan
+        return plan
 
     def __repr__(self):
         return (f"Int8KVCache(num_pages={self.num_pages}, num_heads={self.num_heads}, page_size={self.page_size}, "
                 f"head_dim={self.head_dim}, device={self.device})")
 
-    # ---- argument checks -------------------------------------------------------------------
-    def _tokens(self, t: torch.Tensor, name: str) -> int:
+    # ---- argument checks: once per layout of the arguments -----------------------------------
+    def _check_tokens(self, t: torch.Tensor, name: str) -> int:
         """Checks a [sequences, tokens, heads, head_dim] input; returns its dtype code."""
         if not t.is_cuda:
             raise RuntimeError("aimet_b200 operates on CUDA tensors only; there is no CPU fallback")
@@ -104,17 +115,22 @@ class Int8KVCache:
             raise RuntimeError(f"{name} is on {t.device}, the cache on {self.device}")
         return code
 
-    def _table(self, table: torch.Tensor, seqs: int) -> torch.Tensor:
+    def _check_table(self, table: torch.Tensor, seqs: int) -> None:
         if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != seqs or table.device != self.device:
             raise RuntimeError(f"block_table must be int32 of shape ({seqs}, blocks) on {self.device}, got {table.dtype} of shape "
                                f"{tuple(table.shape)} on {table.device}")
-        return table if table.stride(1) == 1 or table.shape[1] <= 1 else table.contiguous()
 
-    def _lens(self, lens: torch.Tensor, seqs: int, name: str) -> torch.Tensor:
-        if lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != seqs or lens.device != self.device:
+    def _check_lens(self, lens: Optional[torch.Tensor], seqs: int, name: str) -> None:
+        if lens is not None and (lens.dtype != torch.int32 or lens.dim() != 1 or lens.shape[0] != seqs or lens.device != self.device):
             raise RuntimeError(f"{name} must be int32 of shape ({seqs},) on {self.device}, got {lens.dtype} of shape "
                                f"{tuple(lens.shape)} on {lens.device}")
-        return lens if lens.is_contiguous() else lens.contiguous()
+
+    @staticmethod
+    def _dense(table, *lens):
+        """Block table and lengths as the kernels read them: table entries side by side, lengths contiguous."""
+        if table.shape[1] > 1 and table.stride(1) != 1:
+            table = table.contiguous()
+        return table, *(t if t is None or t.is_contiguous() else t.contiguous() for t in lens)
 
     # ---- operators -------------------------------------------------------------------------
     def append(self, key: torch.Tensor, value: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
@@ -132,50 +148,66 @@ class Int8KVCache:
         from finite values.  Tokens whose table entry is outside ``[0, num_pages)``, or lies behind the
         table's end, are dropped.  Within a call no page may receive tokens of two sequences.
         """
-        code = self._tokens(key, "key")
+        signature = ("append", _signature(key), _signature(value), _signature(block_table), _signature(context_lens), _signature(new_lens))
+        plan = self._plans.get(signature) or self._plan_append(signature, key, value, block_table, context_lens, new_lens)
+        if torch.is_grad_enabled() and (key.requires_grad or value.requires_grad):
+            raise RuntimeError("append has no backward pass: call it under torch.no_grad()")
+        code, key_strides, value_strides, dense = plan
+        if not dense:
+            block_table, context_lens, new_lens = self._dense(block_table, context_lens, new_lens)
+            if key_strides is None:
+                key, value = key.contiguous(), value.contiguous()
+                key_strides = value_strides = _Strides(*key.stride()[:3])
+        with _lib.on_device(self.device):
+            check(lib.aimet_b200_kv_append(
+                self._ref, key.data_ptr(), value.data_ptr(), key_strides, value_strides, key.shape[0], key.shape[1],
+                block_table.data_ptr(), block_table.stride(0), block_table.shape[1], context_lens.data_ptr(),
+                None if new_lens is None else new_lens.data_ptr(), code, _lib.stream_ptr(self.device)))
+
+    def _plan_append(self, signature, key, value, table, context, new):
+        code = self._check_tokens(key, "key")
         if value.dtype != key.dtype or value.shape != key.shape or value.device != key.device:
             raise RuntimeError(f"value must be {key.dtype} of shape {tuple(key.shape)} on {key.device}, got {value.dtype} of shape "
                                f"{tuple(value.shape)} on {value.device}")
         if key.shape[2] != self.num_heads:
             raise RuntimeError(f"key has {key.shape[2]} heads, the cache {self.num_heads}")
-        if _needs_grad(key, value):
-            raise RuntimeError("append has no backward pass: call it under torch.no_grad()")
-        seqs, tokens = key.shape[:2]
-        table = self._table(block_table, seqs)
-        context = self._lens(context_lens, seqs, "context_lens")
-        new = None if new_lens is None else self._lens(new_lens, seqs, "new_lens")
-        if key.stride(3) != 1:
-            key = key.contiguous()
-        if value.stride(3) != 1:
-            value = value.contiguous()
-        with _lib.on_device(self.device):
-            check(lib.aimet_b200_kv_append(
-                self._desc, key.data_ptr(), value.data_ptr(), _Strides(*key.stride()[:3]), _Strides(*value.stride()[:3]), seqs,
-                tokens, table.data_ptr(), table.stride(0), table.shape[1], context.data_ptr(), _lib.ptr(new), code,
-                _lib.stream_ptr(self.device)))
+        self._check_table(table, key.shape[0])
+        self._check_lens(context, key.shape[0], "context_lens")
+        self._check_lens(new, key.shape[0], "new_lens")
+        rows = key.stride(3) == 1 and value.stride(3) == 1
+        same = self._dense(table, context, new)
+        dense = rows and same[0] is table and same[1] is context and same[2] is new
+        strides = (_Strides(*key.stride()[:3]), _Strides(*value.stride()[:3])) if rows else (None, None)
+        return self._remember(signature, (code, *strides, dense))
 
     def gather(self, block_table: torch.Tensor, lens: torch.Tensor, length: Optional[int] = None,
                dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys and values ``[sequences, length, num_heads, head_dim]`` of the first ``lens`` (int32) tokens
         of every sequence, zeros behind; ``length`` defaults to all that the table can hold."""
+        signature = ("gather", _signature(block_table), _signature(lens), length, dtype)
+        code, shape = self._plans.get(signature) or self._plan_gather(signature, block_table, lens, length, dtype)
+        block_table, lens = self._dense(block_table, lens)
+        key = torch.empty(shape, dtype=dtype, device=self.device)
+        value = torch.empty_like(key)
+        if key.numel():
+            with _lib.on_device(self.device):
+                check(lib.aimet_b200_kv_gather(self._ref, key.data_ptr(), value.data_ptr(), shape[0], shape[1], block_table.data_ptr(),
+                                               block_table.stride(0), block_table.shape[1], lens.data_ptr(), code,
+                                               _lib.stream_ptr(self.device)))
+        return key, value
+
+    def _plan_gather(self, signature, table, lens, length, dtype):
         code = _lib.DTYPE_CODE.get(dtype)
         if code is None or code == _lib.AB_F64:
             raise NotImplementedError(f"gather gives float32, float16 or bfloat16, not {dtype}")
-        seqs = block_table.shape[0] if block_table.dim() == 2 else -1
-        table = self._table(block_table, seqs)
-        lens = self._lens(lens, seqs, "lens")
+        seqs = table.shape[0] if table.dim() == 2 else -1
+        self._check_table(table, seqs)
+        self._check_lens(lens, seqs, "lens")
         if length is None:
             length = table.shape[1] * self.page_size
         if length < 0:
             raise RuntimeError(f"length={length} is negative")
-        shape = (seqs, length, self.num_heads, self.head_dim)
-        key = torch.empty(shape, dtype=dtype, device=self.device)
-        value = torch.empty(shape, dtype=dtype, device=self.device)
-        if key.numel():
-            with _lib.on_device(self.device):
-                check(lib.aimet_b200_kv_gather(self._desc, key.data_ptr(), value.data_ptr(), seqs, length, table.data_ptr(),
-                                               table.stride(0), table.shape[1], lens.data_ptr(), code, _lib.stream_ptr(self.device)))
-        return key, value
+        return self._remember(signature, (code, (seqs, length, self.num_heads, self.head_dim)))
 
     def attention(self, query: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
                   query_lens: Optional[torch.Tensor] = None, *, causal: bool = True, window: Optional[int] = None,
@@ -194,32 +226,47 @@ class Int8KVCache:
         softmax sum, float32 ``[sequences, tokens, heads]`` (-inf where it sees nothing), by which results
         over parts of a context can be joined.
         """
-        code = self._tokens(query, "query")
-        if _needs_grad(query):
+        signature = ("attention", _signature(query), _signature(block_table), _signature(context_lens), _signature(query_lens), window)
+        plan = self._plans.get(signature) or self._plan_attention(signature, query, block_table, context_lens, query_lens, window)
+        if torch.is_grad_enabled() and query.requires_grad:
             raise RuntimeError("attention over the cache has no backward pass: call it under torch.no_grad()")
+        code, strides, group, need, dense = plan
+        if not dense:
+            block_table, context_lens, query_lens = self._dense(block_table, context_lens, query_lens)
+            if strides is None:
+                query = query.contiguous()
+                strides = _Strides(*query.stride()[:3])
+        seqs, tokens, heads, dim = shape = query.shape
+        out = query.new_empty(shape)
+        lse = query.new_empty((seqs, tokens, heads), dtype=torch.float32) if return_lse else None
+        if need >= 0:  # there are queries
+            with _lib.on_device(self.device):
+                # from the caching allocator, call by call: buffers of two streams, or of two captured graphs,
+                # are never shared
+                part = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+                check(lib.aimet_b200_kv_attention(
+                    self._ref, query.data_ptr(), strides, out.data_ptr(), None if lse is None else lse.data_ptr(), seqs, tokens, group,
+                    block_table.data_ptr(), block_table.stride(0), block_table.shape[1], context_lens.data_ptr(),
+                    None if query_lens is None else query_lens.data_ptr(), causal, window or 0, dim ** -0.5 if scale is None else scale,
+                    code, None if part is None else part.data_ptr(), need, _lib.stream_ptr(self.device)))
+        return (out, lse) if return_lse else out
+
+    def _plan_attention(self, signature, query, table, context, new, window):
+        code = self._check_tokens(query, "query")
         seqs, tokens, heads = query.shape[:3]
         if heads < 1 or heads % self.num_heads:
             raise RuntimeError(f"{heads} query heads are no multiple of the cache's {self.num_heads}")
         if window is not None and window < 1:
             raise RuntimeError(f"window={window}: at least 1, or None for no window")
-        table = self._table(block_table, seqs)
-        context = self._lens(context_lens, seqs, "context_lens")
-        new = None if query_lens is None else self._lens(query_lens, seqs, "query_lens")
-        if query.stride(3) != 1:
-            query = query.contiguous()
-        out = torch.empty((seqs, tokens, heads, self.head_dim), dtype=query.dtype, device=self.device)
-        lse = torch.empty((seqs, tokens, heads), dtype=torch.float32, device=self.device) if return_lse else None
-        if out.numel():
-            group, width = heads // self.num_heads, table.shape[1]
+        self._check_table(table, seqs)
+        self._check_lens(context, seqs, "context_lens")
+        self._check_lens(new, seqs, "query_lens")
+        rows = query.stride(3) == 1
+        same = self._dense(table, context, new)
+        dense = rows and same[0] is table and same[1] is context and same[2] is new
+        group, need = heads // self.num_heads, -1
+        if seqs and tokens:
             with _lib.on_device(self.device):
-                need = lib.aimet_b200_kv_attention_scratch_bytes(self._desc, seqs, tokens, group, width, code)
-                check(need)
-                # from the caching allocator, call by call: buffers of two streams, or of two captured graphs,
-                # are never shared
-                part = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-                check(lib.aimet_b200_kv_attention(
-                    self._desc, query.data_ptr(), _Strides(*query.stride()[:3]), out.data_ptr(), _lib.ptr(lse), seqs, tokens, group,
-                    table.data_ptr(), table.stride(0), width, context.data_ptr(), _lib.ptr(new), int(causal), window or 0,
-                    self.head_dim ** -0.5 if scale is None else float(scale), code, _lib.ptr(part), need,
-                    _lib.stream_ptr(self.device)))
-        return (out, lse) if return_lse else out
+                need = lib.aimet_b200_kv_attention_scratch_bytes(self._ref, seqs, tokens, group, table.shape[1], code)
+            check(need)
+        return self._remember(signature, (code, _Strides(*query.stride()[:3]) if rows else None, group, need, dense))
