@@ -22,6 +22,8 @@ from ._lib import check, lib
 __all__ = ["PackedInt4Weight", "linear_int4"]
 
 _TILE_N, _TILE_K, _CHUNK_K = 16, 64, 256
+# input features of the longest row that the kernels take
+MOST_FEATURES = {torch.float32: 37120, torch.float16: 111360, torch.bfloat16: 111360}
 _MOST_PLANS = 512  # input layouts that a weight remembers
 _MAX_ZERO = 112  # 16-bit floats subtract zero points up to here exactly
 
@@ -100,6 +102,9 @@ class PackedInt4Weight:
         """Bytes on the device."""
         return sum(t.numel() * t.element_size() for t in self._buffers if t is not None)
 
+    def __deepcopy__(self, memo):
+        return self  # its contents are fixed
+
     def __repr__(self):
         return (f"PackedInt4Weight({self.out_features}x{self.in_features}, block_size={self.block_size}, "
                 f"device={self.device})")
@@ -167,6 +172,8 @@ class PackedInt4Weight:
             with _lib.on_device(codes.device):
                 check(lib.aimet_b200_int4_pack(codes8.data_ptr(), n, k, qmin, storage, packed.data_ptr(),
                                                _lib.stream_ptr(codes.device)))
+                # products request weights before they wait for what precedes them in their stream
+                torch.cuda.current_stream(codes.device).synchronize()
         return cls(n, k, block, qmin, packed, scales, int_scale is not None, zeros, row_scale, zero)
 
     @classmethod
@@ -214,8 +221,11 @@ class PackedInt4Weight:
 def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[torch.Tensor] = None) -> torch.Tensor:  # pylint: disable=redefined-builtin
     """``input @ w.T + bias`` for a packed weight: ``[..., in_features] -> [..., out_features]``.
 
-    float32, float16 or bfloat16 activations; sums in float32, one rounding to ``input.dtype``.  For
-    inference: an input or bias that needs a gradient is refused (train through the quantizer instead).
+    float32, float16 or bfloat16 activations; sums in float32, one rounding to ``input.dtype``.  A few
+    tokens, and float32 always, multiply the integer codes exactly; many tokens multiply weights that are
+    rounded to the 16-bit type once, as a simulated 16-bit model's are.  Rows of up to 37120 input features in
+    float32 and 111360 in 16 bits.  For inference: an input or bias that needs a gradient is refused (train
+    through the quantizer instead).
     """
     signature = (input.shape, input.stride(), input.dtype, input.device)
     plan = weight._plans.get(signature)  # pylint: disable=protected-access

@@ -82,7 +82,7 @@ class Int8KVCache:
             raise NotImplementedError(f"head_dim={head_dim}: a multiple of 16 up to 256 is supported")
 
     def _adopt(self, key, value, key_scale, value_scale):
-        self.key, self.value, self.key_scale, self.value_scale = key, value, key_scale, value_scale
+        self._buffers = (key, value, key_scale, value_scale)  # what the descriptor below points at
         self.num_pages, self.num_heads, self.page_size, self.head_dim = key.shape
         self.device = key.device
         self._desc = _lib.KVCache(key.data_ptr(), value.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(),
@@ -96,6 +96,11 @@ class Int8KVCache:
             self._plans.clear()
         self._plans[signature] = plan
         return plan
+
+    key = property(lambda self: self._buffers[0])
+    value = property(lambda self: self._buffers[1])
+    key_scale = property(lambda self: self._buffers[2])
+    value_scale = property(lambda self: self._buffers[3])
 
     def __repr__(self):
         return (f"Int8KVCache(num_pages={self.num_pages}, num_heads={self.num_heads}, page_size={self.page_size}, "

@@ -18,7 +18,7 @@ import torch
 from torch import nn
 
 from .encoding_analyzer import MinMaxEncodingAnalyzer
-from .int4 import PackedInt4Weight, linear_int4
+from .int4 import MOST_FEATURES, PackedInt4Weight, linear_int4
 from .quantizer import QuantizeDequantize
 
 __all__ = ["QuantizedLayer", "quantize_model", "compute_encodings", "quantized_layers", "precomputed"]
@@ -190,7 +190,9 @@ def _allreduce_minmax_statistics(quantizers, group):
 def _packable(layer: QuantizedLayer) -> bool:
     """A Linear layer whose weight quantizer has a grid of at most 4 bits that the packed layout can hold."""
     qw = layer.param_quantizers["weight"]
-    return isinstance(layer.layer, nn.Linear) and qw is not None and qw.is_initialized() and qw.qmax - qw.qmin <= 15
+    weight = layer.layer.weight
+    return (isinstance(layer.layer, nn.Linear) and qw is not None and qw.is_initialized() and qw.qmax - qw.qmin <= 15
+            and weight.numel() > 0 and weight.shape[1] <= MOST_FEATURES.get(weight.dtype, 0))
 
 
 @contextlib.contextmanager

@@ -420,7 +420,9 @@ int aimet_b200_int4_pack(const void *codes, int64_t n, int64_t k, int qmin, int 
  * ldy; bias (io_dtype, n elements) may be NULL.  Float32 accumulation, one rounding to io_dtype.  Few
  * tokens, float32, and rows of x that do not start on 16 bytes: codes are multiplied exactly.  Otherwise
  * a tensor-core kernel multiplies weights rounded to io_dtype; *status (int32 that the device can write,
- * may be pinned host memory) becomes non-zero if one of its bounded waits gives up. */
+ * may be pinned host memory) becomes non-zero if one of its bounded waits gives up.  The weight's buffers
+ * are read before the kernel waits for its predecessor in the stream (programmatic dependent launch):
+ * whatever writes them has to be complete when this is called. */
 int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *x, int64_t ldx, const void *bias, void *y,
                            int64_t ldy, int64_t tokens, int io_dtype, int32_t *status, void *stream);
 

@@ -284,6 +284,37 @@ def test_refusals():
         PackedInt4Weight.from_codes(codes[:0], scale[:0], None, qmin=0)
 
 
+def test_a_wait_that_gave_up_is_reported_by_the_next_call():
+    """The status word is written here by hand: nothing makes a kernel wait."""
+    from aimet_b200 import int4
+
+    parts = make(48, 64, 64, "sym")
+    p = packed_of(*parts)
+    x = torch.randn(64, 64, device="cuda").half()
+    want = int4.linear_int4(x, p)
+    int4._status._words[torch.cuda.current_device()][1].value = 2
+    with pytest.raises(RuntimeError, match="gave up waiting"):
+        int4.linear_int4(x, p)
+    assert torch.equal(int4.linear_int4(x, p), want)
+
+
+def test_longest_rows():
+    """The most input features of float32, and 16-bit rows of which one token at a time fits shared memory; longer
+    ones are refused."""
+    from aimet_b200.int4 import MOST_FEATURES, PackedInt4Weight, linear_int4
+
+    for dtype, k in ((torch.float32, MOST_FEATURES[torch.float32]), (torch.bfloat16, 60000), (torch.float16, MOST_FEATURES[torch.float16])):
+        codes = torch.randint(-8, 8, (20, k), device="cuda", dtype=torch.int8)
+        scale = torch.rand(20, 1, device="cuda") + 0.1
+        p = PackedInt4Weight.from_codes(codes, scale)
+        for tokens in (1, 2, 3, 40):
+            x = torch.randn(tokens, k, device="cuda").to(dtype) * 0.01
+            assert_close(linear_int4(x, p), x, dequantized(codes, scale, None, None), weight_in_16=tokens > 2 and dtype != torch.float32)
+    p = PackedInt4Weight.from_codes(torch.zeros(16, MOST_FEATURES[torch.float16] + 1, device="cuda"), torch.ones(16, 1, device="cuda"))
+    with pytest.raises(NotImplementedError, match="shared memory"):
+        linear_int4(torch.zeros(1, p.in_features, device="cuda", dtype=torch.half), p)
+
+
 def test_zero_points_beyond_the_grid():
     """Offsets need not lie on the grid: every whole zero point up to 112 is subtracted exactly."""
     from aimet_b200.int4 import linear_int4
