@@ -251,7 +251,7 @@ _HERE = _Here()
 def on_device(device: torch.device):
     """Context in which ``device`` is the current CUDA device (kernels are launched on the current
     device): nothing to switch, and nothing to pay, in the usual case that it already is."""
-    if device.index is None or device.index == torch._C._cuda_getDevice():  # pylint: disable=protected-access
+    if device.index is None or device.index == torch.cuda.current_device():
         return _HERE
     return torch.cuda.device(device)
 

@@ -54,6 +54,10 @@ def _tiled(param: torch.Tensor, block: int, storage: int, in_features: int) -> t
     return out.view(-1, _TILE_N, chunks, entries, sub).permute(0, 2, 3, 1, 4).contiguous()
 
 
+_current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
+_current_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
+
+
 class _Status:
     """The word that a kernel's bounded waits write when they give up, per device, in pinned host memory:
     looked at by the next call without waiting for the device."""
@@ -61,8 +65,7 @@ class _Status:
     def __init__(self):
         self._words: dict[int, tuple[torch.Tensor, ctypes.c_int32]] = {}
 
-    def pointer(self, device: torch.device) -> int:
-        index = device.index if device.index is not None else torch.cuda.current_device()
+    def pointer(self, index: int) -> int:
         held = self._words.get(index)
         if held is None:
             word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
@@ -94,7 +97,9 @@ class PackedInt4Weight:
                                      codes.data_ptr(), scales.data_ptr(), _lib.ptr(zeros), row_scale.data_ptr())
         self.device = codes.device
         self._ref = ctypes.byref(self._desc)
-        _status.pointer(self.device)  # made now: a first product may be inside a stream capture, where it could not be
+        self._index = codes.get_device()
+        _status.pointer(self._index)  # made now: a first product may be inside a stream capture, where it could not be
+        self._bias_shape = torch.Size((out_features,))
         self._plans: dict = {}  # layout of an input -> what follows from it
 
     @property
@@ -227,7 +232,7 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
     float32 and 111360 in 16 bits.  For inference: an input or bias that needs a gradient is refused (train
     through the quantizer instead).
     """
-    signature = (input.shape, input.stride(), input.dtype, input.device)
+    signature = (input.shape, input.stride(), input.dtype, input.get_device())
     plan = weight._plans.get(signature)  # pylint: disable=protected-access
     if plan is None:
         plan = _plan_linear(signature, input, weight)
@@ -235,10 +240,11 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
         raise RuntimeError("linear_int4 has no backward pass: call it under torch.no_grad(), or train through the weight's quantizer")
     code, tokens, pitch, out_shape, direct, watched = plan
     if bias is not None:
-        if bias.dtype != input.dtype or bias.device != input.device or tuple(bias.shape) != (weight.out_features,):
+        if bias.dtype != input.dtype or bias.get_device() != input.get_device() or bias.shape != weight._bias_shape:  # pylint: disable=protected-access
             raise RuntimeError(f"bias must be {input.dtype} of shape {(weight.out_features,)} on {input.device}, "
                                f"got {bias.dtype} of shape {tuple(bias.shape)} on {bias.device}")
-        bias = bias.contiguous()
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
     out = input.new_empty(out_shape)
     if tokens == 0:
         return out
@@ -248,10 +254,15 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
         pitch = -(-weight.in_features // 8) * 8
         rows = input.reshape(tokens, weight.in_features)
         input = rows.new_empty(tokens, pitch)[:, : weight.in_features].copy_(rows)
-    status = _status.pointer(weight.device) if watched else None
-    with _lib.on_device(weight.device):
-        check(lib.aimet_b200_int4_linear(weight._ref, input.data_ptr(), pitch, None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
-                                         weight.out_features, tokens, code, status, _lib.stream_ptr(weight.device)))
+    index = weight._index  # pylint: disable=protected-access
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return linear_int4(input.reshape(out_shape[:-1] + (weight.in_features,)), weight, bias)
+    rc = lib.aimet_b200_int4_linear(weight._ref, input.data_ptr(), pitch, None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
+                                    weight.out_features, tokens, code, _status.pointer(index) if watched else None,
+                                    _current_stream(index))
+    if rc:
+        check(rc)
     return out
 
 

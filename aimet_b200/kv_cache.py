@@ -25,9 +25,8 @@ _Strides = ctypes.c_int64 * 3
 _MOST_PLANS = 512  # checked argument layouts that a cache remembers
 
 
-def _signature(t: Optional[torch.Tensor]):
-    """What the checks of an argument depend on (nothing of its values or address)."""
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+_current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
+_current_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
 
 
 class Int8KVCache:
@@ -153,7 +152,11 @@ class Int8KVCache:
         from finite values.  Tokens whose table entry is outside ``[0, num_pages)``, or lies behind the
         table's end, are dropped.  Within a call no page may receive tokens of two sequences.
         """
-        signature = ("append", _signature(key), _signature(value), _signature(block_table), _signature(context_lens), _signature(new_lens))
+        # what the checks of the arguments depend on (nothing of their values or addresses)
+        signature = (key.shape, key.stride(), key.dtype, key.get_device(), value.shape, value.stride(), value.dtype, value.get_device(),
+                     block_table.shape, block_table.stride(), block_table.dtype, block_table.get_device(), context_lens.shape,
+                     context_lens.stride(), context_lens.dtype, context_lens.get_device(),
+                     new_lens if new_lens is None else (new_lens.shape, new_lens.stride(), new_lens.dtype, new_lens.get_device()))
         plan = self._plans.get(signature) or self._plan_append(signature, key, value, block_table, context_lens, new_lens)
         if torch.is_grad_enabled() and (key.requires_grad or value.requires_grad):
             raise RuntimeError("append has no backward pass: call it under torch.no_grad()")
@@ -163,11 +166,16 @@ class Int8KVCache:
             if key_strides is None:
                 key, value = key.contiguous(), value.contiguous()
                 key_strides = value_strides = _Strides(*key.stride()[:3])
-        with _lib.on_device(self.device):
-            check(lib.aimet_b200_kv_append(
-                self._ref, key.data_ptr(), value.data_ptr(), key_strides, value_strides, key.shape[0], key.shape[1],
-                block_table.data_ptr(), block_table.stride(0), block_table.shape[1], context_lens.data_ptr(),
-                None if new_lens is None else new_lens.data_ptr(), code, _lib.stream_ptr(self.device)))
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.append(key, value, block_table, context_lens, new_lens)
+        seqs, tokens = key.shape[:2]
+        rc = lib.aimet_b200_kv_append(
+            self._ref, key.data_ptr(), value.data_ptr(), key_strides, value_strides, seqs, tokens, block_table.data_ptr(),
+            block_table.stride(0), block_table.shape[1], context_lens.data_ptr(), None if new_lens is None else new_lens.data_ptr(), code,
+            _current_stream(self._index))
+        if rc:
+            check(rc)
 
     def _plan_append(self, signature, key, value, table, context, new):
         code = self._check_tokens(key, "key")
@@ -189,16 +197,19 @@ class Int8KVCache:
                dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys and values ``[sequences, length, num_heads, head_dim]`` of the first ``lens`` (int32) tokens
         of every sequence, zeros behind; ``length`` defaults to all that the table can hold."""
-        signature = ("gather", _signature(block_table), _signature(lens), length, dtype)
+        signature = (block_table.shape, block_table.stride(), block_table.dtype, block_table.get_device(), lens.shape, lens.stride(),
+                     lens.dtype, lens.get_device(), length, dtype)
         code, shape = self._plans.get(signature) or self._plan_gather(signature, block_table, lens, length, dtype)
         block_table, lens = self._dense(block_table, lens)
-        key = torch.empty(shape, dtype=dtype, device=self.device)
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.gather(block_table, lens, length, dtype)
+        key = lens.new_empty(shape, dtype=dtype)
         value = torch.empty_like(key)
-        if key.numel():
-            with _lib.on_device(self.device):
-                check(lib.aimet_b200_kv_gather(self._ref, key.data_ptr(), value.data_ptr(), shape[0], shape[1], block_table.data_ptr(),
-                                               block_table.stride(0), block_table.shape[1], lens.data_ptr(), code,
-                                               _lib.stream_ptr(self.device)))
+        rc = lib.aimet_b200_kv_gather(self._ref, key.data_ptr(), value.data_ptr(), shape[0], shape[1], block_table.data_ptr(),
+                                      block_table.stride(0), block_table.shape[1], lens.data_ptr(), code, _current_stream(self._index))
+        if rc:
+            check(rc)
         return key, value
 
     def _plan_gather(self, signature, table, lens, length, dtype):
@@ -231,7 +242,10 @@ class Int8KVCache:
         softmax sum, float32 ``[sequences, tokens, heads]`` (-inf where it sees nothing), by which results
         over parts of a context can be joined.
         """
-        signature = ("attention", _signature(query), _signature(block_table), _signature(context_lens), _signature(query_lens), window)
+        signature = (query.shape, query.stride(), query.dtype, query.get_device(), block_table.shape, block_table.stride(),
+                     block_table.dtype, block_table.get_device(), context_lens.shape, context_lens.stride(), context_lens.dtype,
+                     context_lens.get_device(), window,
+                     query_lens if query_lens is None else (query_lens.shape, query_lens.stride(), query_lens.dtype, query_lens.get_device()))
         plan = self._plans.get(signature) or self._plan_attention(signature, query, block_table, context_lens, query_lens, window)
         if torch.is_grad_enabled() and query.requires_grad:
             raise RuntimeError("attention over the cache has no backward pass: call it under torch.no_grad()")
@@ -241,19 +255,24 @@ class Int8KVCache:
             if strides is None:
                 query = query.contiguous()
                 strides = _Strides(*query.stride()[:3])
+        if _current_device() != self._index:
+            with torch.cuda.device(self._index):
+                return self.attention(query, block_table, context_lens, query_lens, causal=causal, window=window, scale=scale,
+                                      return_lse=return_lse)
         seqs, tokens, heads, dim = shape = query.shape
         out = query.new_empty(shape)
         lse = query.new_empty((seqs, tokens, heads), dtype=torch.float32) if return_lse else None
         if need >= 0:  # there are queries
-            with _lib.on_device(self.device):
-                # from the caching allocator, call by call: buffers of two streams, or of two captured graphs,
-                # are never shared
-                part = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-                check(lib.aimet_b200_kv_attention(
-                    self._ref, query.data_ptr(), strides, out.data_ptr(), None if lse is None else lse.data_ptr(), seqs, tokens, group,
-                    block_table.data_ptr(), block_table.stride(0), block_table.shape[1], context_lens.data_ptr(),
-                    None if query_lens is None else query_lens.data_ptr(), causal, window or 0, dim ** -0.5 if scale is None else scale,
-                    code, None if part is None else part.data_ptr(), need, _lib.stream_ptr(self.device)))
+            # scratch from the caching allocator, call by call: buffers of two streams, or of two captured graphs, are
+            # never shared
+            part = query.new_empty(need, dtype=torch.uint8) if need else None
+            rc = lib.aimet_b200_kv_attention(
+                self._ref, query.data_ptr(), strides, out.data_ptr(), None if lse is None else lse.data_ptr(), seqs, tokens, group,
+                block_table.data_ptr(), block_table.stride(0), block_table.shape[1], context_lens.data_ptr(),
+                None if query_lens is None else query_lens.data_ptr(), causal, window or 0, dim ** -0.5 if scale is None else scale, code,
+                None if part is None else part.data_ptr(), need, _current_stream(self._index))
+            if rc:
+                check(rc)
         return (out, lse) if return_lse else out
 
     def _plan_attention(self, signature, query, table, context, new, window):
