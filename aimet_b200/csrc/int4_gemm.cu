@@ -13,8 +13,10 @@
 // operand (`bn` = 32 .. 256 columns).  A stage holds 64 input channels: x comes by TMA, the weights are
 // converted, a warp for each 16-channel tile of the packed layout, and stored in
 // the 128-byte-swizzled order that tcgen05.mma reads: a lane's eight neighbouring columns are one 16-byte
-// store.  Per stage of 256 tokens the MMAs take 524 clocks, the conversion about 300 issue
-// slots of an SM's four schedulers: the tensor cores are the limit.
+// store.  What bounds it: a stage of 256 tokens is 524 clocks of MMAs, and about 640 of conversion (1500 x 14336 x
+// 4096: 160 us, 1.10 PFLOP/s; 134 us with the conversion's loads taken out).  Tried and not kept: a pair of CTAs that
+// each convert half of the channels and store them into both shared memories (304 us: four stages do not cover
+// the way of a store, a fence and an arrival to the other SM).
 //
 // Roles (768 threads): warp 0 TMA, warp 1 TMEM and MMA issue, warps 4-19 conversion (sixteen, in two turns: a
 // warp's chain of a stage, from the barrier to the fence, is long), warps 20-23 epilogue.
@@ -265,7 +267,9 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
                                         out[e][r][p] = fma2(v, hi, mul2(v, lo, E()), E());
                                     }
                                 }
-                        stage += first + kt - at;  // at most three further: fewer than there are stages
+                        // at most three further (a last chunk with one tile): a warp that skipped more than a ring of stages could
+                        // not tell one that is two uses behind from a free one
+                        stage += first + kt - at;
                         at = first + kt;
                         if (stage >= a.stages) stage -= a.stages, phase ^= 1;
                         ok = mbar_wait(bar_empty + 8 * stage, phase ^ 1, abort_flag, a.status, ST4_CONVERT, a.timeout_ns);

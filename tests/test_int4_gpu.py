@@ -98,6 +98,27 @@ def test_many_tokens(dtype, grid, tokens, n, k, block):
     assert_close(got, x, dequantized(codes, scale, offset, int_scale), bias, weight_in_16=dtype != torch.float32)
 
 
+# more tiles than SMs, so that a CTA walks several: odd and even numbers of token tiles, a last chunk with one
+# column tile and with all four, every block class
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("grid,tokens,n,k,block", [
+    ("asym", 513, 6400, 576, 64), ("lpbq", 700, 6300, 320, 32), ("sym", 300, 9500, 272, 16), ("asym", 1024, 5000, 256, 128),
+    ("sym", 2000, 2500, 1040, 0), ("asym", 257, 9600, 1024, 32),
+])
+def test_many_tiles(dtype, grid, tokens, n, k, block):
+    from aimet_b200.int4 import linear_int4
+
+    parts = make(n, k, block, grid, seed=tokens)
+    codes, scale, offset, _, int_scale = parts
+    x = torch.randn(tokens, k, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    bias = torch.randn(n, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    p, w = packed_of(*parts), dequantized(codes, scale, offset, int_scale)
+    one = linear_int4(x, p, bias)
+    assert_close(one, x, w, bias, weight_in_16=True)
+    for _ in range(10):
+        assert torch.equal(one, linear_int4(x, p, bias))
+
+
 @pytest.mark.parametrize("tokens", [3, 70])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_strides_alignment_and_leading_dims(dtype, tokens):
