@@ -9,7 +9,9 @@
 // 16-bit floats (a shift and one three-input logic operation put the code into the mantissa of 128
 // (bfloat16) or 1024 (float16); subtracting 128 + z or 1024 + z is exact) and multiplied 16 x 8 x 16
 // at a time by mma.sync with the weights as the 16-row operand and up to eight tokens as the 8 columns
-// (tcgen05 has 64 rows at least, and the tensor cores are 12 % busy as it is).
+// (tcgen05 has 64 rows at least, and the tensor cores are 16 % busy as it is).  Measured, 1 x 14336 x 4096 with
+// blocks of 64: 10.1 us of 4.7 (3.0 TB/s); issue slots 52 % taken while an SM is active, a third of a launch
+// by itself is ramp-up and tail, which a neighbouring launch overlaps.
 // Products of a 16-bit activation with an integer below 2^8 are exact, sums are float32; every 64
 // columns (or smaller blocks) the sums are multiplied by the block's scale and added up in float32.
 // A float32 activation is cut into three bfloat16 terms that together hold all its 24 bits, each

@@ -15,6 +15,8 @@
 // (movmatrix).  More rows are further columns that share the converted codes.  The scales
 // never touch an element: a tile of 16 tokens lies in one page, so the key scale multiplies the scores,
 // and log2 of the value scale is added to the exponent of the weights that multiply V.
+// Measured: 64 contexts of 1000 to 4000 tokens, 8 heads of 128 for 32 query heads, 90 us of 55 (3.9 TB/s; 135 with query
+// rows as the 16-row operand), 2 of 131072 tokens 98 us of 71 (4.7 TB/s); issue slots 58 % taken.
 //
 // Precision: q is scaled by a power of two per row into float16's range (exact for float16 and
 // bfloat16; what a bfloat16 row loses below 2^-39 of its largest element does not reach a float32 sum);

@@ -34,7 +34,8 @@ __host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b 
 // already keeps its scale while that covers the new tokens and otherwise takes max(that, 1.25 * scale), its codes becoming rint(code * (old / new)).  Growing by a quarter at
 // least bounds what repeated rounding can add up to: half a step each time, 2.5 final steps in all.
 //
-// Bound by reading the new tokens and writing a byte for each element.  x / scale is the correctly rounded
+// Bound by reading the new tokens and writing a byte for each element (4 x up to 2000 tokens, 8 heads of 128, float16: 18 us of
+// 7 by itself, most of it the chain lengths - table - page of small blocks).  x / scale is the correctly rounded
 // quotient without the divide unit: r = 1 / s, q0 = x * r, q = q0 + r * (x - q0 * s) with fused
 // multiply-adds (Markstein's theorem; scales outside [2^-100, 2^100] are divided by the divide unit).
 // ---------------------------------------------------------------------------------------------------
