@@ -665,7 +665,7 @@ template <typename E> __global__ void __launch_bounds__(kJoinWarps * 32) k_kv_jo
     if (a.lse && threadIdx.x == 0) a.lse[at] = dead ? -CUDART_INF_F : (top + log2f(l)) * 0.69314718055994531f;
 }
 
-// how a call is cut: row blocks of 8, 16 or 32 rows, pieces along the cache
+// how a call is cut: row blocks of 8 or 16 rows, pieces along the cache
 struct Cut {
     int eights, row_blocks, pieces, target;
     bool cluster;  // the pieces of a row block are a cluster of CTAs; otherwise they leave partial results in scratch
@@ -674,20 +674,21 @@ int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens, int64_t table_width, int io_dtype) {
     Cut c;
     const int64_t rows = tokens * group;
-    // more rows per CTA share the converted codes; O and Q of 32 rows do not fit the registers for wider heads,
-    // nor for float32's two terms
-    c.eights = rows <= 8 ? 1 : rows <= 16 || padded_dim(dim) > 128 || io_dtype == AB_F32 ? 2 : 4;
+    // Sixteen rows per CTA share the converted codes.  (Thirty-two leave registers for two CTAs of four warps on an SM
+    // and lost: 35 rows of dim 64 over 1500 tokens 27 us against 20, 64 rows of dim 128 over 4000 134 against 100.)
+    c.eights = rows <= 8 ? 1 : 2;
     c.row_blocks = (int)std::min<int64_t>(div_up(rows, 8 * c.eights), 1 << 20);
     const int64_t length = table_width * page;
     // CTAs on an SM, by registers and shared memory
     const int wide = padded_dim(dim);
-    const int resident = wide == 256 ? 1 : c.eights == 1 ? (wide == 64 ? 5 : 3) : c.eights == 2 && wide == 64 ? 4 : 2;
+    const int resident = wide == 256 ? 1 : c.eights == 1 ? (wide == 64 ? 5 : 3) : wide == 64 ? 4 : 2;
     const int64_t slots = (int64_t)sm_count() * resident, base = std::max<int64_t>(1, seqs * heads * c.row_blocks);
     const int64_t want = slots * (base >= slots / 2 ? kWaves : 1);
     c.target = (int)std::max<int64_t>(1, want / std::max<int64_t>(1, (int64_t)heads * c.row_blocks));
     // Eight pieces or fewer, or contexts that eight CTAs are not long over, are joined through the cluster's shared
     // memory (one launch, no scratch): one of 500 tokens 5.9 us, 7.9 us as two launches.
-    const int64_t wanted = div_up(want, base), most = std::max<int64_t>(1, div_up(length, kMinPiece));
+    // (where pieces fill the machine, no more than one wave of them: 16 of 1000 tokens 13.6 us, 18.2 with a few more)
+    const int64_t wanted = base >= slots / 2 ? div_up(want, base) : std::max<int64_t>(1, want / base), most = std::max<int64_t>(1, div_up(length, kMinPiece));
     c.cluster = std::min(wanted, most) <= kMostCluster || length <= kMostCluster * kClusterPiece;
     // otherwise a sequence may be cut four times finer than evenly long ones would be
     c.pieces = (int)(c.cluster ? std::min<int64_t>(kMostCluster, std::min(wanted, most)) : std::min(most, 4 * wanted));
@@ -743,9 +744,6 @@ template <typename E, int DP, int NQ> int launch(const AttnArgs &a, cudaStream_t
 }
 template <typename E> int dispatch(const AttnArgs &a, int eights, cudaStream_t st) {
     const int dp = padded_dim(a.dim);
-    if constexpr (sizeof(E) == 2) {
-        if (eights == 4) return dp == 64 ? launch<E, 64, 4>(a, st) : launch<E, 128, 4>(a, st);
-    }
     if (eights == 2) return dp == 64 ? launch<E, 64, 2>(a, st) : dp == 128 ? launch<E, 128, 2>(a, st) : launch<E, 256, 2>(a, st);
     return dp == 64 ? launch<E, 64, 1>(a, st) : dp == 128 ? launch<E, 128, 1>(a, st) : launch<E, 256, 1>(a, st);
 }
