@@ -275,3 +275,18 @@ class _Scratch:
 
 
 scratch = _Scratch()
+
+
+def _load_calls():
+    """The extension module that makes the per-token operators' plain calls (``csrc/calls.cpp``), or None where it
+    was not built for this Python and torch: the Python code makes the same calls, at more host time."""
+    try:
+        from . import _calls
+    except ImportError:
+        return None
+    names = ("int4_linear", "kv_append", "kv_gather", "kv_attention", "kv_attention_scratch_bytes")
+    _calls.init(*(ctypes.cast(getattr(lib, "aimet_b200_" + n), ctypes.c_void_p).value for n in names))
+    return _calls
+
+
+calls = _load_calls()

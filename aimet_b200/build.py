@@ -1,6 +1,7 @@
-"""Builds ``libaimet_b200.so`` (the C-ABI kernel library) in-tree with nvcc for sm_100a.
+"""Builds ``libaimet_b200.so`` (the C-ABI kernel library) in-tree with nvcc for sm_100a, and the extension
+module ``_calls.so`` (host code of the per-token operators) with the host compiler.
 
-Usage: ``python -m aimet_b200.build [--force] [--verbose]``.  The library is written next to
+Usage: ``python -m aimet_b200.build [--force] [--verbose]``.  Both are written next to
 this file; nothing is cached outside the source tree.
 """
 
@@ -17,6 +18,8 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 SRC_DIR = os.path.join(PKG_DIR, "csrc")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 LIB_PATH = os.path.join(PKG_DIR, "libaimet_b200.so")
+CALLS_SRC = os.path.join(SRC_DIR, "calls.cpp")
+CALLS_PATH = os.path.join(PKG_DIR, "_calls.so")  # the Python extension module aimet_b200._calls
 STAMP_PATH = LIB_PATH + ".stamp"
 
 NVCC_FLAGS = [
@@ -42,7 +45,10 @@ def _source_digest() -> str:
     """Hash of everything the library is made from: the sources, the public header, the flags."""
     import hashlib
 
+    from importlib.metadata import version
+
     h = hashlib.sha256(" ".join(NVCC_FLAGS).encode())
+    h.update((version("torch") + sys.version).encode())  # what the extension module is compiled against
     paths = sorted(os.path.join(SRC_DIR, f) for f in os.listdir(SRC_DIR))
     paths.append(os.path.join(PKG_DIR, os.pardir, "include", "aimet_b200.h"))
     for p in paths:
@@ -55,10 +61,29 @@ def _source_digest() -> str:
 def is_up_to_date() -> bool:
     """True when the library on disk was built from exactly the present sources (by content, not by
     file times: a checkout or a copy to another machine changes times but not contents)."""
-    if not (os.path.exists(LIB_PATH) and os.path.exists(STAMP_PATH)):
+    if not (os.path.exists(LIB_PATH) and os.path.exists(CALLS_PATH) and os.path.exists(STAMP_PATH)):
         return False
     with open(STAMP_PATH) as f:
         return f.read().strip() == _source_digest()
+
+
+def _build_calls() -> None:
+    """The extension module: host code over torch's C++ interface and the C ABI header."""
+    import sysconfig
+
+    import torch
+
+    torch_dir = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    tmp = CALLS_PATH + ".tmp"
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",  # pylint: disable=protected-access
+           "-I" + os.path.join(torch_dir, "include"), "-I" + os.path.join(torch_dir, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"), CALLS_SRC, "-o", tmp,
+           "-L" + os.path.join(torch_dir, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed for {CALLS_SRC}:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, CALLS_PATH)
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
@@ -80,7 +105,9 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return obj
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        calls = pool.submit(_build_calls)
         objs = list(pool.map(compile_one, _sources()))
+        calls.result()
 
     tmp = LIB_PATH + ".tmp"
     cmd = [nvcc, "-shared", "-o", tmp, *objs, "-gencode", "arch=compute_100a,code=sm_100a", "-cudart", "static"]

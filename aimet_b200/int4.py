@@ -54,6 +54,7 @@ def _tiled(param: torch.Tensor, block: int, storage: int, in_features: int) -> t
     return out.view(-1, _TILE_N, chunks, entries, sub).permute(0, 2, 3, 1, 4).contiguous()
 
 
+_calls = _lib.calls
 _current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
 _current_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
 
@@ -65,12 +66,14 @@ class _Status:
     def __init__(self):
         self._words: dict[int, tuple[torch.Tensor, ctypes.c_int32]] = {}
 
-    def pointer(self, index: int) -> int:
-        held = self._words.get(index)
-        if held is None:
+    def address(self, index: int) -> int:
+        if index not in self._words:
             word = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-            held = self._words[index] = (word, ctypes.c_int32.from_address(word.data_ptr()))
-        word, value = held
+            self._words[index] = (word, ctypes.c_int32.from_address(word.data_ptr()))
+        return self._words[index][0].data_ptr()
+
+    def checked(self, index: int) -> int:
+        word, value = self._words[index]
         if value.value:
             code, value.value = value.value, 0
             raise RuntimeError(f"aimet_b200: an earlier linear_int4 call on cuda:{index} gave up waiting (device status {code}); "
@@ -98,7 +101,8 @@ class PackedInt4Weight:
         self.device = codes.device
         self._ref = ctypes.byref(self._desc)
         self._index = codes.get_device()
-        _status.pointer(self._index)  # made now: a first product may be inside a stream capture, where it could not be
+        self._address = ctypes.addressof(self._desc)
+        self._status = _status.address(self._index)  # made now: a first product may be inside a stream capture, where it could not be
         self._bias_shape = torch.Size((out_features,))
         self._plans: dict = {}  # layout of an input -> what follows from it
 
@@ -232,6 +236,10 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
     float32 and 111360 in 16 bits.  For inference: an input or bias that needs a gradient is refused (train
     through the quantizer instead).
     """
+    if _calls is not None:
+        out = _calls.linear(input, bias, weight._address, weight._index, weight._status)  # pylint: disable=protected-access
+        if out is not None:
+            return out
     signature = (input.shape, input.stride(), input.dtype, input.get_device())
     plan = weight._plans.get(signature)  # pylint: disable=protected-access
     if plan is None:
@@ -259,7 +267,7 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
         with torch.cuda.device(index):
             return linear_int4(input.reshape(out_shape[:-1] + (weight.in_features,)), weight, bias)
     rc = lib.aimet_b200_int4_linear(weight._ref, input.data_ptr(), pitch, None if bias is None else bias.data_ptr(), out.data_ptr(),  # pylint: disable=protected-access
-                                    weight.out_features, tokens, code, _status.pointer(index) if watched else None,
+                                    weight.out_features, tokens, code, _status.checked(index) if watched else None,
                                     _current_stream(index))
     if rc:
         check(rc)

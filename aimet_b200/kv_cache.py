@@ -25,6 +25,7 @@ _Strides = ctypes.c_int64 * 3
 _MOST_PLANS = 512  # checked argument layouts that a cache remembers
 
 
+_calls = _lib.calls
 _current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
 _current_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
 
@@ -87,6 +88,8 @@ class Int8KVCache:
         self._desc = _lib.KVCache(key.data_ptr(), value.data_ptr(), key_scale.data_ptr(), value_scale.data_ptr(),
                                   self.num_pages, self.num_heads, self.page_size, self.head_dim, 0)
         self._ref = ctypes.byref(self._desc)
+        self._address = ctypes.addressof(self._desc)
+        self._scale = self.head_dim ** -0.5
         self._index = self.device.index if self.device.index is not None else torch.cuda.current_device()
         self._plans: dict = {}  # signature of a call's arguments -> what follows from it
 
@@ -152,6 +155,8 @@ class Int8KVCache:
         from finite values.  Tokens whose table entry is outside ``[0, num_pages)``, or lies behind the
         table's end, are dropped.  Within a call no page may receive tokens of two sequences.
         """
+        if _calls is not None and _calls.append(key, value, block_table, context_lens, new_lens, self._address, self._index):
+            return
         # what the checks of the arguments depend on (nothing of their values or addresses)
         signature = (key.shape, key.stride(), key.dtype, key.get_device(), value.shape, value.stride(), value.dtype, value.get_device(),
                      block_table.shape, block_table.stride(), block_table.dtype, block_table.get_device(), context_lens.shape,
@@ -197,6 +202,11 @@ class Int8KVCache:
                dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys and values ``[sequences, length, num_heads, head_dim]`` of the first ``lens`` (int32) tokens
         of every sequence, zeros behind; ``length`` defaults to all that the table can hold."""
+        code = _lib.DTYPE_CODE.get(dtype, _lib.AB_F64)
+        if _calls is not None and code != _lib.AB_F64 and (length is None or length >= 0):
+            out = _calls.gather(block_table, lens, -1 if length is None else length, code, self._address, self._index)
+            if out is not None:
+                return out
         signature = (block_table.shape, block_table.stride(), block_table.dtype, block_table.get_device(), lens.shape, lens.stride(),
                      lens.dtype, lens.get_device(), length, dtype)
         code, shape = self._plans.get(signature) or self._plan_gather(signature, block_table, lens, length, dtype)
@@ -242,6 +252,12 @@ class Int8KVCache:
         softmax sum, float32 ``[sequences, tokens, heads]`` (-inf where it sees nothing), by which results
         over parts of a context can be joined.
         """
+        scale = self._scale if scale is None else float(scale)
+        if _calls is not None and (window is None or window >= 1):
+            out = _calls.attention(query, block_table, context_lens, query_lens, causal, window or 0, scale, return_lse, self._address,
+                                   self._index)
+            if out is not None:
+                return out
         signature = (query.shape, query.stride(), query.dtype, query.get_device(), block_table.shape, block_table.stride(),
                      block_table.dtype, block_table.get_device(), context_lens.shape, context_lens.stride(), context_lens.dtype,
                      context_lens.get_device(), window,
@@ -259,8 +275,8 @@ class Int8KVCache:
             with torch.cuda.device(self._index):
                 return self.attention(query, block_table, context_lens, query_lens, causal=causal, window=window, scale=scale,
                                       return_lse=return_lse)
-        seqs, tokens, heads, dim = shape = query.shape
-        out = query.new_empty(shape)
+        seqs, tokens, heads = query.shape[:3]
+        out = query.new_empty(query.shape)
         lse = query.new_empty((seqs, tokens, heads), dtype=torch.float32) if return_lse else None
         if need >= 0:  # there are queries
             # scratch from the caching allocator, call by call: buffers of two streams, or of two captured graphs, are
@@ -269,7 +285,7 @@ class Int8KVCache:
             rc = lib.aimet_b200_kv_attention(
                 self._ref, query.data_ptr(), strides, out.data_ptr(), None if lse is None else lse.data_ptr(), seqs, tokens, group,
                 block_table.data_ptr(), block_table.stride(0), block_table.shape[1], context_lens.data_ptr(),
-                None if query_lens is None else query_lens.data_ptr(), causal, window or 0, dim ** -0.5 if scale is None else scale, code,
+                None if query_lens is None else query_lens.data_ptr(), causal, window or 0, scale, code,
                 None if part is None else part.data_ptr(), need, _current_stream(self._index))
             if rc:
                 check(rc)

@@ -13,6 +13,16 @@ from torch import nn
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(params=["native calls", "python calls"])
+def calls(request, monkeypatch):
+    """The extension module's calls, and the same calls made from Python."""
+    from aimet_b200 import _lib, int4
+
+    assert _lib.calls is not None
+    if request.param == "python calls":
+        monkeypatch.setattr(int4, "_calls", None)
+
+
 def make(n, k, block, grid, seed=0, device="cuda"):
     g = torch.Generator().manual_seed(seed)
     blocks = k // (block or k)
@@ -87,7 +97,7 @@ def test_matches_the_product_in_64_bits(dtype, grid, tokens, n, k, block):
     ("sym", 64, 256, 512, 128), ("asym", 129, 300, 1024, 64), ("lpbq", 257, 130, 768, 32), ("asym", 40, 513, 272, 16),
     ("sym", 100, 128, 333, 0), ("asym", 515, 640, 4096, 128), ("lpbq", 33, 1000, 2048, 256), ("sym", 300, 72, 64, 64),
 ])
-def test_many_tokens(dtype, grid, tokens, n, k, block):
+def test_many_tokens(calls, dtype, grid, tokens, n, k, block):
     from aimet_b200.int4 import linear_int4
 
     parts = make(n, k, block, grid, seed=tokens)
@@ -121,7 +131,7 @@ def test_many_tiles(dtype, grid, tokens, n, k, block):
 
 @pytest.mark.parametrize("tokens", [3, 70])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_strides_alignment_and_leading_dims(dtype, tokens):
+def test_strides_alignment_and_leading_dims(calls, dtype, tokens):
     from aimet_b200.int4 import linear_int4
 
     parts = make(48, 256, 64, "asym")
@@ -174,7 +184,7 @@ def test_rows_keep_to_themselves(tokens):
     assert torch.equal(linear_int4(y, p)[:-1], one[:-1])
 
 
-def test_calls_captured_into_graphs_and_on_other_streams():
+def test_calls_captured_into_graphs_and_on_other_streams(calls):
     from aimet_b200.int4 import linear_int4
 
     parts = make(256, 512, 64, "lpbq")
@@ -228,7 +238,7 @@ def test_packs_what_the_quantizers_calibrate(kind):
         assert p._desc.scale_kind == 1  # the integer factors are kept as bytes
 
 
-def test_model_with_packed_weights():
+def test_model_with_packed_weights(calls):
     """nn.precomputed(model, packed=True): same results as the simulated weights up to the sums' rounding."""
     from aimet_b200 import nn as qnn
 
@@ -267,7 +277,7 @@ def test_model_with_packed_weights():
         assert "_held_weight" in model8[0].__dict__ and "_packed_weight" not in model8[0].__dict__
 
 
-def test_refusals():
+def test_refusals(calls):
     from aimet_b200.int4 import PackedInt4Weight, linear_int4
 
     codes, scale, offset, qmin, _ = make(16, 64, 32, "asym")
@@ -305,7 +315,7 @@ def test_refusals():
         PackedInt4Weight.from_codes(codes[:0], scale[:0], None, qmin=0)
 
 
-def test_a_wait_that_gave_up_is_reported_by_the_next_call():
+def test_a_wait_that_gave_up_is_reported_by_the_next_call(calls):
     """The status word is written here by hand: nothing makes a kernel wait."""
     from aimet_b200 import int4
 
@@ -319,7 +329,7 @@ def test_a_wait_that_gave_up_is_reported_by_the_next_call():
     assert torch.equal(int4.linear_int4(x, p), want)
 
 
-def test_longest_rows():
+def test_longest_rows(calls):
     """The most input features of float32, and 16-bit rows of which one token at a time fits shared memory; longer
     ones are refused."""
     from aimet_b200.int4 import MOST_FEATURES, PackedInt4Weight, linear_int4

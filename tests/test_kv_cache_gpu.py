@@ -20,6 +20,17 @@ pytestmark = pytest.mark.gpu
 LEVELS = 127
 
 
+@pytest.fixture(params=["native calls", "python calls"])
+def calls(request, monkeypatch):
+    """The extension module's calls, and the same calls made from Python."""
+    from aimet_b200 import _lib, int4, kv_cache
+
+    assert _lib.calls is not None
+    if request.param == "python calls":
+        monkeypatch.setattr(int4, "_calls", None)
+        monkeypatch.setattr(kv_cache, "_calls", None)
+
+
 def make_cache(pages, heads, page, dim, seed=0, spread=0.0):
     from aimet_b200.kv_cache import Int8KVCache
 
@@ -130,7 +141,7 @@ def test_single_tokens_over_ragged_contexts(dtype, heads, group, dim, page):
     (2, 3, 64, 16, 5, None, True), (1, 4, 128, 32, 8, 33, True), (1, 7, 64, 16, 5, 1, True), (2, 1, 96, 16, 20, 16, True),
     (1, 6, 128, 64, 11, None, False), (1, 2, 256, 16, 9, 100, True), (1, 16, 64, 16, 16, None, True), (1, 3, 80, 16, 3, 40, False),
 ])
-def test_several_tokens_windows_and_padding(dtype, heads, group, dim, page, tokens, window, causal):
+def test_several_tokens_windows_and_padding(calls, dtype, heads, group, dim, page, tokens, window, causal):
     context = [0, 2, tokens, 40, 257, 500]
     new = [0, tokens, tokens, tokens - 2, tokens, 1]  # the second has more tokens than its context
     cache = make_cache(70, heads, page, dim, seed=tokens)
@@ -213,7 +224,7 @@ def test_queries_of_any_size(size):
         check_attention(cache, q.to(dtype), table, [50], None, scale=0.1 / size)
 
 
-def test_query_strides_and_alignment():
+def test_query_strides_and_alignment(calls):
     cache = make_cache(8, 2, 16, 64)
     table = make_table([70, 40], 16, 8)
     for dtype in (torch.bfloat16, torch.float32):
@@ -315,7 +326,7 @@ def expected_append(cache, key, value, table, context, new):
     (1, 16, 16, [0], [1]), (2, 64, 16, [0, 5, 15, 16, 31], [1, 1, 1, 1, 1]), (2, 128, 64, [0, 63, 64, 10], [70, 2, 130, 0]),
     (1, 80, 32, [7, 0, 33], [100, 32, 31]), (3, 256, 16, [1, 14], [40, 3]), (2, 96, 128, [100, 0], [300, 128]), (1, 48, 48, [47, 48], [2, 49]),
 ])
-def test_append(dtype, heads, dim, page, context, new):
+def test_append(calls, dtype, heads, dim, page, context, new):
     pages = 40
     cache = make_cache(pages, heads, page, dim, seed=page)
     table = make_table([c + n for c, n in zip(context, new)], page, pages)
@@ -384,7 +395,7 @@ def test_append_token_by_token_stays_within_its_bound():
         assert float(((key - x[:, :, 0]).abs() / cache.key_scale[2][:, None]).max()) <= 0.5 + 1e-4
 
 
-def test_append_drops_what_has_no_page():
+def test_append_drops_what_has_no_page(calls):
     cache = make_cache(6, 1, 16, 32)
     table = ints([[0, -1, 2], [6, 3, 2**31 - 1]])
     x = torch.randn(2, 60, 1, 32, device="cuda")
@@ -396,7 +407,7 @@ def test_append_drops_what_has_no_page():
 
 
 # ---------------------------------------------------------------------------------------------- together
-def test_decode_steps_of_a_layer_with_packed_weights_and_the_cache():
+def test_decode_steps_of_a_layer_with_packed_weights_and_the_cache(calls):
     """Prompt, then tokens one by one: projections with packed weights, append, attention, output projection,
     against the same steps in 64 bits on what the cache holds."""
     from test_int4_gpu import assert_close, dequantized, make, packed_of
@@ -427,7 +438,7 @@ def test_decode_steps_of_a_layer_with_packed_weights_and_the_cache():
         assert_close(linear_int4(y, po), y, wo, weight_in_16=y.shape[0] * y.shape[1] > 8)
 
 
-def test_steps_captured_into_graphs_and_replayed_side_by_side():
+def test_steps_captured_into_graphs_and_replayed_side_by_side(calls):
     """Append and attention in one graph each for two caches; both replayed at once, lengths and tokens updated
     between replays; a third cache runs eagerly meanwhile."""
     caches, states = [], []
@@ -468,7 +479,7 @@ def test_steps_captured_into_graphs_and_replayed_side_by_side():
             assert torch.equal(want, graphs[i][1] if i < 2 else eager)
 
 
-def test_refusals():
+def test_refusals(calls):
     from aimet_b200.kv_cache import Int8KVCache
 
     cache = make_cache(4, 2, 16, 32)

@@ -106,6 +106,26 @@ def test_entry_points_refuse_before_touching_the_device():
     assert lib.aimet_b200_kv_attention_scratch_bytes(cache(), 1, 1, 4, 1, _lib.AB_BF16) == 0
 
 
+def test_extension_module_leaves_what_is_not_plain_to_python():
+    """Built with the library; CPU tensors, wrong types and wrong shapes come back as None before anything runs."""
+    from aimet_b200 import _lib
+
+    calls = _lib.calls
+    assert calls is not None
+    w = _lib.Int4Weight(32, 128, 64, 0, 8, 0, None, None, None, None)
+    status = ctypes.c_int32(0)
+    where = (ctypes.addressof(w), 0, ctypes.addressof(status))
+    assert calls.linear(torch.zeros(2, 128), None, *where) is None
+    assert calls.linear("no tensor", None, *where) is None
+    c = _lib.KVCache(None, None, None, None, 10, 2, 16, 64, 0)
+    x, ints = torch.zeros(1, 1, 2, 64), torch.zeros(1, dtype=torch.int32)
+    assert calls.append(x, x, ints[None], ints, None, ctypes.addressof(c), 0) is None
+    assert calls.gather(ints[None], ints, -1, _lib.AB_BF16, ctypes.addressof(c), 0) is None
+    assert calls.attention(x, ints[None], ints, None, True, 0, 0.1, False, ctypes.addressof(c), 0) is None
+    with pytest.raises(TypeError):
+        calls.linear(x)
+
+
 def test_cpu_tensors_are_refused():
     from aimet_b200.int4 import PackedInt4Weight
     from aimet_b200.kv_cache import Int8KVCache
