@@ -83,18 +83,26 @@ PyObject *linear(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int code = code_of(x->scalar_type());
     const int64_t tokens = x->numel() / w->k;
     if (code < 0 || *status) Py_RETURN_NONE;
-    // what the tensor-core kernel would read unaligned is copied first
-    if (tokens > 16 && code != AB_F32 && (w->k % 8 || reinterpret_cast<uintptr_t>(x->data_ptr()) % 16)) Py_RETURN_NONE;
     const void *bias = nullptr;
     if (a[1] != Py_None) {
         const at::Tensor *b = plain(a[1], index);
         if (!b || b->scalar_type() != x->scalar_type() || b->dim() != 1 || b->size(0) != w->n || !b->is_contiguous()) Py_RETURN_NONE;
         bias = b->data_ptr();
     }
-    c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
+    // what the tensor-core kernel would read unaligned is copied first
+    at::Tensor padded;
+    int64_t pitch = w->k;
+    if (tokens > 16 && code != AB_F32 && (w->k % 8 || reinterpret_cast<uintptr_t>(x->data_ptr()) % 16)) {
+        pitch = (w->k + 7) / 8 * 8;
+        padded = at::empty({tokens, pitch}, x->options().requires_grad(false));
+        padded.narrow(1, 0, w->k).copy_(x->detach().view({tokens, w->k}));
+        x = &padded;
+    }
+    const at::Tensor &input = THPVariable_Unpack(a[0]);
+    c10::SmallVector<int64_t, 6> shape(input.sizes().begin(), input.sizes().end());
     shape.back() = w->n;
     at::Tensor y = at::empty(shape, x->options().requires_grad(false));
-    if (g_linear(w, x->data_ptr(), w->k, bias, y.data_ptr(), w->n, tokens, code, const_cast<int32_t *>(status), current_stream(index)) != AB_OK)
+    if (g_linear(w, x->data_ptr(), pitch, bias, y.data_ptr(), w->n, tokens, code, const_cast<int32_t *>(status), current_stream(index)) != AB_OK)
         Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(y));
     BODY_END

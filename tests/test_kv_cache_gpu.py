@@ -273,7 +273,7 @@ def test_results_do_not_depend_on_the_run_or_on_other_sequences():
 
 # ------------------------------------------------------------------------------------------ append, gather
 def expected_append(cache, key, value, table, context, new):
-    """Checks a cache in place against what append must have made of `before`: returns a checker."""
+    """Checks a cache in place against what append must have made of `before`: returns that check."""
     before = {n: getattr(cache, n).clone() for n in ("key", "value", "key_scale", "value_scale")}
     page = cache.page_size
 
