@@ -138,6 +138,7 @@ PyObject *gather(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const int64_t index = integer(a[5]);
     int64_t length = integer(a[2]);
     const int code = (int)integer(a[3]);
+    if (PyErr_Occurred()) return nullptr;
     const at::Tensor *l = plain(a[1], index);
     if (!l || l->dim() != 1 || l->size(0) == 0 || !current(index)) Py_RETURN_NONE;
     const int64_t seqs = l->size(0);
@@ -169,7 +170,7 @@ PyObject *attention(PyObject *, PyObject *const *a, Py_ssize_t n) {
     const at::Tensor *t = block_table(a[1], index, seqs), *ctx = lengths(a[2], index, seqs);
     const at::Tensor *len = a[3] == Py_None ? nullptr : lengths(a[3], index, seqs);
     if (!t || !ctx || (a[3] != Py_None && !len)) Py_RETURN_NONE;
-    const int causal = PyObject_IsTrue(a[4]), with_lse = PyObject_IsTrue(a[7]);
+    const int causal = PyObject_IsTrue(a[4]), with_lse = PyObject_IsTrue(a[7]);  // (-1 with an error set)
     const int64_t window = integer(a[5]);
     const double scale = PyFloat_AsDouble(a[6]);
     if (PyErr_Occurred()) return nullptr;

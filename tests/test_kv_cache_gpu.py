@@ -12,6 +12,8 @@ attention: with p the exact softmax, an output is off by at most the sum of
 * what weights below float16's normal range lose: 2^-25 of the largest p |v scale| * 127, per token.
 """
 
+import ctypes
+
 import pytest
 import torch
 
@@ -522,6 +524,13 @@ def test_refusals(calls):
         cache.attention(x[..., :16], table, lens)
     with pytest.raises(NotImplementedError, match="int8"):
         cache.gather(table, lens, dtype=torch.int8)
+    for bad in (5.0, "5"):
+        with pytest.raises((TypeError, RuntimeError)):
+            cache.gather(table, lens, bad)
+    with pytest.raises((TypeError, RuntimeError, ctypes.ArgumentError)):
+        cache.attention(x, table, lens, window=2.5)
+    with pytest.raises((TypeError, ValueError)):
+        cache.attention(x, table, lens, scale="big")
     # nothing to do
     empty = torch.randn(0, 1, 2, 32, device="cuda")
     cache.append(empty, empty, table[:0], lens[:0])
