@@ -15,8 +15,8 @@
 // (movmatrix).  More rows are further columns that share the converted codes.  The scales
 // never touch an element: a tile of 16 tokens lies in one page, so the key scale multiplies the scores,
 // and log2 of the value scale is added to the exponent of the weights that multiply V.
-// Measured: 64 contexts of 1000 to 4000 tokens, 8 heads of 128 for 32 query heads, 90 us of 55 (3.9 TB/s; 135 with query
-// rows as the 16-row operand), 2 of 131072 tokens 98 us of 71 (4.7 TB/s); issue slots 58 % taken.
+// Measured: 64 contexts of 1000 to 4000 tokens, 8 heads of 128 for 32 query heads, 87 us of 55 (4.0 TB/s; 135 with query
+// rows as the 16-row operand), 2 of 131072 tokens 98 to 101 us of 71 (4.6 TB/s); issue slots 58 % taken.
 //
 // Precision: q is scaled by a power of two per row into float16's range (exact for float16 and
 // bfloat16; what a bfloat16 row loses below 2^-39 of its largest element does not reach a float32 sum);
@@ -128,25 +128,20 @@ template <int DP> __device__ __forceinline__ uint32_t place_v(int row, int byte)
     return at ^ (((row >> 1) & 3) << 5);
 }
 
-// 16 consecutive elements of a query row as floats, zeros beyond the row's end
-template <typename E> __device__ __forceinline__ void load_row16(const E *p, int left, bool vec, float (&f)[16]) {
+// 16 consecutive elements of a query row
+template <typename E> struct Sixteen {
+    Vec16<E> v[sizeof(E)];
+};
+template <typename E> __device__ __forceinline__ void load_row16(const E *p, bool vec, Sixteen<E> &x) {
     constexpr int V = 16 / sizeof(E);
-    if (left <= 0) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[i] = 0.f;
-        return;
-    }
-    // dim is a multiple of 16, so there are 16 elements or none
+    for (int j = 0; j < (int)sizeof(E); ++j) {
+        if (vec) {
+            x.v[j] = *reinterpret_cast<const Vec16<E> *>(p + j * V);
+        } else {
 #pragma unroll
-    for (int j = 0; j < 16 / V; ++j) {
-        Vec16<E> v;
-        if (vec)
-            v = *reinterpret_cast<const Vec16<E> *>(p + j * V);
-        else
-#pragma unroll
-            for (int i = 0; i < V; ++i) v.v[i] = p[j * V + i];
-#pragma unroll
-        for (int i = 0; i < V; ++i) f[j * V + i] = to_f32(v.v[i]);
+            for (int i = 0; i < V; ++i) x.v[j].v[i] = p[j * V + i];
+        }
     }
 }
 
@@ -237,13 +232,24 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int piece = blockIdx.x, h = blockIdx.y / a.row_blocks, rb = blockIdx.y % a.row_blocks, s = blockIdx.z;
+    const int rows = a.tokens * a.group;  // of the output
+    const int row0 = rb * L::kRows;
     pdl_prologue();
+
+    // this lane's part of query row g of every eight, requested before anything is known of the lengths
+    Sixteen<E> raw[NQ][NC];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int r = row0 + 8 * n + g, token = r / a.group, gq = r - token * a.group;
+        const E *p = static_cast<const E *>(a.q) + (int64_t)s * a.q_seq + (int64_t)token * a.q_tok + (int64_t)(h * a.group + gq) * a.q_head;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if (r < rows && 64 * c + 16 * t < a.dim) load_row16(p + 64 * c + 16 * t, a.vec, raw[n][c]);
+    }
 
     const int cap = (int)min((long long)a.table_width * a.page, 0x7fffffffll);
     const int ctx = min(max(a.context[s], 0), cap);
     const int len = a.qlens ? min(max(a.qlens[s], 0), a.tokens) : a.tokens;
-    const int rows = a.tokens * a.group;                    // of the output
-    const int row0 = rb * L::kRows;
     const int live = min(max(len * a.group - row0, 0), L::kRows);  // rows of this block with a query
     const int first_token = row0 / a.group, last_token = (row0 + live - 1) / a.group;
     Span span = {0, 0};
@@ -323,25 +329,25 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
         next = w[kStages - 1];
     }
 
-    // the queries as operand fragments: this lane's part of query row g of every eight
+    // the queries as operand fragments
     uint32_t qf[NQ][QS][NC][4][2];
     float score_scale[NQ][2];             // of rows 2t, 2t + 1 of the eight, as everything below
     int lo_row[NQ][2], hi_row[NQ][2];
     int max_lo = 0, min_hi = 0x7fffffff;
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int r = 8 * n + g;
-        const bool alive = r < live;
-        const int token = alive ? (row0 + r) / a.group : 0, gq = alive ? (row0 + r) % a.group : 0;
-        const E *p = static_cast<const E *>(a.q) + (int64_t)s * a.q_seq + (int64_t)token * a.q_tok + (int64_t)(h * a.group + gq) * a.q_head;
+        const bool alive = 8 * n + g < live;
         float top = 0.f;
         float f[NC][16];
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int d = 64 * c + 16 * t;
-            load_row16(p + d, alive ? a.dim - d : 0, a.vec, f[c]);
+            const bool here = alive && 64 * c + 16 * t < a.dim;  // (dim is a multiple of 16: all sixteen or none)
+            constexpr int V = 16 / sizeof(E);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(f[c][e]));
+            for (int e = 0; e < 16; ++e) {
+                f[c][e] = here ? to_f32(raw[n][c].v[e / V].v[e % V]) : 0.f;
+                top = fmaxf(top, fabsf(f[c][e]));
+            }
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -687,7 +693,7 @@ Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens
     c.target = (int)std::max<int64_t>(1, want / std::max<int64_t>(1, (int64_t)heads * c.row_blocks));
     // Eight pieces or fewer, or contexts that eight CTAs are not long over, are joined through the cluster's shared
     // memory (one launch, no scratch): one of 500 tokens 5.9 us, 7.9 us as two launches.
-    // (where pieces fill the machine, no more than one wave of them: 16 of 1000 tokens 13.6 us, 18.2 with a few more)
+    // (where pieces fill the machine, no more than one wave of them: 16 of 1000 tokens 12.3 us; 18.2 against 13.6 with a few more)
     const int64_t wanted = base >= slots / 2 ? div_up(want, base) : std::max<int64_t>(1, want / base), most = std::max<int64_t>(1, div_up(length, kMinPiece));
     c.cluster = std::min(wanted, most) <= kMostCluster || length <= kMostCluster * kClusterPiece;
     // otherwise a sequence may be cut four times finer than evenly long ones would be
