@@ -82,8 +82,11 @@ __device__ __forceinline__ void pdl_prologue() {
     pdl_wait();
 }
 
-// all threads of a cluster's CTAs; what was written to shared memory before is visible to all after
+// All threads of a cluster's CTAs; what was written to shared memory before is visible to all after.  The aligned
+// form has to be executed by a warp's lanes together, which a loop with a trip count for each lane, or a
+// conditional store, does not leave behind by itself.
 __device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 

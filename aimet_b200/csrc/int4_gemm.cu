@@ -335,11 +335,13 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (live && c + j < left) y[(int64_t)(c + j) * a.ldy] = Cvt<float, E>::store(fmaf(__uint_as_float(ra[j]), f, b));
+                    __syncwarp();  // (reading tensor memory is a warp's lanes together, after stores that some lanes skip)
                     tmem_ld_wait();
                     if (c + 32 < a.bn) tmem_ld16(t0 + c + 32, ra);
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
                         if (live && c + 16 + j < left) y[(int64_t)(c + 16 + j) * a.ldy] = Cvt<float, E>::store(fmaf(__uint_as_float(rb[j]), f, b));
+                    __syncwarp();
                 }
             }
             tc_fence_before();

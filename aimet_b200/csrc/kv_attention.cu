@@ -316,6 +316,7 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
                 cp_async16(dst + L::kTile + place_v<DP>(r, copy_chunk * 16), vp + j * copy_step, bytes);
             }
             if (lane < 2) cp_async4(dst + 2 * L::kTile + 4 * lane, scale + ph, there ? 4 : 0);
+            __syncwarp();  // (the products that follow are a warp's lanes together)
         }
         cp_commit();
     };

@@ -330,7 +330,7 @@ k_seqmse(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUten
     }
     tc_fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync_all();  // the partner's barriers are initialised before anything signals them
+    if (PAIR) cluster_barrier();  // the partner's barriers are initialised before anything signals them
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
     const unsigned long long limit = a.timeout_ns;
@@ -540,7 +540,7 @@ k_seqmse(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUten
     // (in a pair: in both CTAs, so neither leaves while the other may still signal its barriers)
     tc_fence_before();
     __syncthreads();
-    if (PAIR) cluster_sync_all();
+    if (PAIR) cluster_barrier();
     tc_fence_after();
     if (warp == 1) {
         if (PAIR)
