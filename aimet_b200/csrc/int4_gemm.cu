@@ -144,7 +144,9 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
             }
         }
     } else if (warp == 1) {
-        // the whole warp walks the loop and one elected lane issues a stage as straight-line code
+        // The whole warp walks the loop and one elected lane issues a stage as straight-line code.  The limit of its
+        // waits counts from the predecessor's end, before which no stage can be filled.
+        pdl_wait();
         int stage = 0;
         uint32_t phase = 0, pass = 0;
         bool ok = true;

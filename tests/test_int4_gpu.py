@@ -357,3 +357,48 @@ def test_zero_points_beyond_the_grid():
     for dtype in (torch.bfloat16, torch.float16, torch.float32):
         x = torch.randn(3, 128, device="cuda").to(dtype)
         assert_close(linear_int4(x, p), x, w)
+
+
+def test_a_slow_predecessor_is_not_a_wait_that_gave_up():
+    """The tensor-core kernel may become resident while its predecessor in the stream still runs; the limit of its
+    waits (two seconds) counts from the predecessor's end.  The predecessor here is attention of one query over
+    one page that a table names again and again, by one CTA (the other sequences hold nothing but leave no
+    more than one CTA for each), for three seconds or so."""
+    from aimet_b200 import _lib, int4
+    from aimet_b200.kv_cache import Int8KVCache
+
+    cache = Int8KVCache(1, 1, 1024, 16)
+    seqs = 4096
+    q = torch.randn(seqs, 1, 1, 16, device="cuda").half()
+    blocks = (1 << 30) // 1024
+    table = torch.zeros(1, blocks, dtype=torch.int32, device="cuda").expand(seqs, blocks)
+    context = torch.zeros(seqs, dtype=torch.int32, device="cuda")
+
+    def timed(tokens):
+        context[0] = tokens
+        torch.cuda.synchronize()
+        start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        cache.attention(q, table, context)
+        stop.record()
+        torch.cuda.synchronize()
+        return start.elapsed_time(stop)
+
+    timed(1 << 20)
+    per_token = timed(1 << 23) / (1 << 23)
+    parts = make(512, 256, 64, "sym")
+    p = packed_of(*parts)
+    x = torch.randn(64, 256, device="cuda").half()
+    want = int4.linear_int4(x, p)
+    context[0] = min((1 << 30) - 1, int(3000 / per_token))
+    torch.cuda.synchronize()
+    assert _lib.lib.aimet_b200_kv_attention_scratch_bytes(cache._ref, seqs, 1, 1, blocks, _lib.AB_F16) == 0  # one kernel, nothing behind it
+    start, stop = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    cache.attention(q, table, context)
+    got = int4.linear_int4(x, p)
+    stop.record()
+    torch.cuda.synchronize()
+    assert start.elapsed_time(stop) > 2200, "the predecessor has to take longer than the limit"
+    assert torch.equal(got, want)
+    assert torch.equal(int4.linear_int4(x, p), want)  # and nothing is reported
