@@ -84,6 +84,19 @@ class _Status:
 _status = _Status()
 
 
+def _simulated_codes(weight: torch.Tensor, encoding) -> torch.Tensor:
+    """The codes whose values ``quantize_dequantize`` gives for a weight when no gradient is wanted.  That is what
+    ``quantize`` gives, except where the fake-quantize arithmetic runs (per tensor and per channel): there the
+    weight is multiplied by 1 / scale in float32 whatever its type, while ``quantize`` divides in the weight's
+    type, and quotients near the middle of two codes (in bfloat16 one of a hundred) fall differently."""
+    scale, offset, qmin, qmax, block = encoding.scale, encoding.offset, encoding.qmin, encoding.qmax, encoding.block_size
+    if not backend._takes_fake_quantize_path(weight, scale, offset, block, 0.0, qmin, qmax):  # pylint: disable=protected-access
+        return backend.quantize(weight, scale, offset, qmin, qmax, block)
+    # (code + offset) * scale in float32, |code + offset| <= 15: the quotient is off by 2^-20 at most
+    value = backend.quantize_dequantize(weight.to(torch.float32), scale, offset, qmin, qmax, block)
+    return torch.round(value / scale) - offset
+
+
 class PackedInt4Weight:
     """4-bit codes of a linear layer's weight with their scales, laid out for the CUDA kernels.
 
@@ -188,7 +201,8 @@ class PackedInt4Weight:
     @classmethod
     def from_encoding(cls, weight: torch.Tensor, encoding) -> "PackedInt4Weight":
         """Quantize ``weight`` ``[out_features, in_features]`` with a 4-bit ``AffineEncoding`` (per tensor, per
-        output channel, or blockwise along the input channels) and pack the codes."""
+        output channel, or blockwise along the input channels) and pack the codes: the ones that
+        ``quantize_dequantize`` simulates when no gradient is wanted."""
         if weight.dim() != 2:
             raise NotImplementedError(f"weights of linear layers are packed, got shape {tuple(weight.shape)}")
         if encoding.qmax - encoding.qmin > 15:
@@ -198,9 +212,9 @@ class PackedInt4Weight:
         n, k = weight.shape
         scale, offset = encoding.scale, encoding.offset
         with torch.no_grad():
-            codes = backend.quantize(weight.detach(), scale, offset, encoding.qmin, encoding.qmax, encoding.block_size)
             if scale.dim() > 2:
                 raise NotImplementedError(f"scales of shape {tuple(scale.shape)} for a linear layer's weight")
+            codes = _simulated_codes(weight.detach(), encoding)
 
             def per_channel(p):  # [out or 1, blocks] -> [out, blocks]
                 p = p.detach().to(torch.float32).reshape((1,) * (2 - p.dim()) + tuple(p.shape))

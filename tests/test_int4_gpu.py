@@ -402,3 +402,79 @@ def test_a_slow_predecessor_is_not_a_wait_that_gave_up():
     assert start.elapsed_time(stop) > 2200, "the predecessor has to take longer than the limit"
     assert torch.equal(got, want)
     assert torch.equal(int4.linear_int4(x, p), want)  # and nothing is reported
+
+
+def linear_bound(x, w, bias, out_dtype, weights_in_16):
+    """How far two results y = x . w^T + bias may be apart: each is rounded to its type once, sums float32 (as
+    in assert_close); `weights_in_16` of the two multiply weights that are rounded to 16 bits."""
+    xd = x.double()
+    y, size = xd @ w.T, xd.abs() @ w.abs().T
+    if bias is not None:
+        y, size = y + bias.double(), size + bias.double().abs()
+    half = torch.finfo(out_dtype).eps / 2
+    sums = (w.shape[1] / 16 + 32) * 2.0**-23 * size
+    return 2 * half * y.abs() + (2 * sums + weights_in_16 * half * size) * (1 + half) + 2.0**-24
+
+
+def layers_of(dtype, seed=0, sizes=((64, 96, True), (96, 40, False)), grid="per_channel"):
+    """Linear layers with calibrated 4-bit weight quantizers and no activation quantizers."""
+    from aimet_b200 import nn as qnn
+    from aimet_b200.quantizer import GroupedBlockQuantizeDequantize, QuantizeDequantize
+
+    def quantizer(n, k):
+        if grid == "lpbq":
+            return GroupedBlockQuantizeDequantize((n, k // 32), 4, True, 8, block_size=(1, 32), block_grouping=(1, k // 32))
+        shape, block = {"per_channel": ((n, 1), None), "asymmetric": ((n, 1), None), "per_tensor": ((), None)}.get(grid, ((n, k // 16), (1, 16)))
+        return QuantizeDequantize(shape, 4, grid != "asymmetric", block_size=block)
+
+    torch.manual_seed(seed)
+    model = nn.Sequential(*[qnn.QuantizedLayer(nn.Linear(k, n, bias=b), None, None, quantizer(n, k)) for k, n, b in sizes])
+    model = model.to("cuda", dtype).eval()
+    for layer in model:
+        with layer.param_quantizers["weight"].compute_encodings():
+            layer.param_quantizers["weight"](layer.layer.weight)
+    return model
+
+
+@pytest.mark.parametrize("grid", ["per_channel", "per_tensor", "asymmetric", "blockwise", "lpbq"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_packed_codes_are_the_simulated_ones(dtype, grid):
+    """What a packed weight stands for, read through a product with the unit matrix, against the simulated weight:
+    apart by roundings (of the scale, the product and the read-back, half a step each), never by a code."""
+    from aimet_b200.int4 import PackedInt4Weight, linear_int4
+
+    for layer in layers_of(dtype, grid=grid, sizes=((256, 384, False), (96, 40, False))):
+        quantizer, weight = layer.param_quantizers["weight"], layer.layer.weight
+        with torch.no_grad():
+            simulated = quantizer(weight).double()
+            eye = torch.eye(weight.shape[1], device="cuda")
+            packed = linear_int4(eye, PackedInt4Weight.from_quantizer(weight, quantizer)).double().T
+        half = torch.finfo(dtype).eps / 2
+        assert bool(((packed - simulated).abs() <= (2 * half * (1 + half) + 2.0**-22) * packed.abs()).all())
+        scale = quantizer.get_encodings().scale.detach().double()
+        assert float(simulated.abs().max()) > 3 * float(scale.min())  # (steps are far wider than that)
+
+
+@pytest.mark.parametrize("grid", ["per_channel", "per_tensor", "asymmetric", "blockwise", "lpbq"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [1, 7, 40, 300])
+def test_packed_weights_against_the_weights_held_otherwise(dtype, tokens, grid):
+    """precomputed(packed=True) and precomputed() on the same layer, from one token to a prompt."""
+    from aimet_b200 import nn as qnn
+
+    model = layers_of(dtype, grid=grid)
+    x = torch.randn(tokens, 64, device="cuda").to(dtype)
+    with torch.no_grad():
+        for layer in model:
+            with qnn.precomputed(model):
+                want, w = layer(x), layer._held_weight.double()
+            with qnn.precomputed(model, packed=True):
+                assert "_packed_weight" in layer.__dict__
+                got = layer(x)
+            assert got.dtype == want.dtype == dtype
+            # the held weight is rounded to the type, its scale too where blocks have one, and many tokens round the packed one
+            bound = linear_bound(x, w, layer.layer.bias, dtype, 0 if dtype == torch.float32 else 3)
+            if dtype == torch.float32:  # (code + offset) * scale rounded to float32: half a step of each weight
+                bound = bound + 2.0**-23 * (x.double().abs() @ w.abs().T)
+            assert bool(((got.double() - want.double()).abs() <= bound).all())
+            x = want
