@@ -21,11 +21,15 @@
 // Precision: q is scaled by a power of two per row into float16's range (exact for float16 and
 // bfloat16; what a bfloat16 row loses below 2^-39 of its largest element does not reach a float32 sum);
 // float32 queries are cut into two float16 terms (22 bits).  Scores, maxima, sums and O are float32.
-// The weights are rounded to float16 for the second product (11 bits, at most 2^-11 of a weight, where a
-// bfloat16 or float16 output is itself rounded to 2^-8 or 2^-11); float32 outputs take two terms.
+// The weights are rounded to float16 for the second product, scaled by 2^15 so that the largest lies in the
+// upper end of its range: at most 2^-11 of a weight is lost (where a bfloat16 or float16 output is itself
+// rounded to 2^-8 or 2^-11), 2^-22 where float32 outputs take two terms, and below 2^-29 of the largest weight times
+// value scale, where float16 has no more normal numbers, 2^-40 of that largest.
 //
-// Two running maxima: m of the scores (for the sum of weights), mv of score + log2(value scale) (for the
-// weighted sum of codes), so a page whose values are large or small against the others' loses nothing.
+// Two running maxima: m of the scores (for the sum of weights), mv of score - m + log2(value scale) (for the
+// weighted sum of codes, whose unit is 2^(m + mv - 15)), so a page whose values are large or small against the
+// others' loses nothing.  mv is relative to m: both sums take a token's weight from the same difference score - m, and
+// stay consistent where scores are so large that m + log2(value scale) would not hold the second term.
 //
 // Split: every warp works alone on tiles of 16 tokens, kStages of them in flight in its own part of
 // shared memory (cp.async), and keeps its own maxima, sums and O; a CTA's warps are joined through
@@ -51,6 +55,9 @@ constexpr int kMinPiece = 128, kMaxMinPiece = 512;
 // two); three where sequences and heads do, so that ragged lengths even out (64 of 1000 to 4000: 99 us, 106 with one).
 constexpr int kWaves = 3;
 constexpr int kMostCluster = 8, kClusterPiece = 1024;
+
+constexpr float kWeightExponent = 15.f, kWeightDown = 1.f / 32768.f;  // weights are multiplied as 2^15 times themselves
+constexpr float kLeastUnit = -126.f;  // of mv: values that are nothing beside float32's smallest normal number make no unit of their own
 
 struct AttnArgs {
     const int8_t *key, *value;
@@ -400,7 +407,7 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) m[n][i] = mv[n][i] = -CUDART_INF_F, sum[n][i] = 0.f;
+        for (int i = 0; i < 2; ++i) m[n][i] = -CUDART_INF_F, mv[n][i] = kLeastUnit, sum[n][i] = 0.f;
 #pragma unroll
         for (int d = 0; d < DP / 16; ++d)
 #pragma unroll
@@ -464,14 +471,17 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
 #pragma unroll
                 for (int w = 4; w <= 16; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
                 const float m1 = fmaxf(m[n][r], top), ref = m1 == -CUDART_INF_F ? 0.f : m1;
-                sum[n][r] = sum[n][r] * exp2_fast(m[n][r] - ref) + (exp2_fast(x0 - ref) + exp2_fast(x1 - ref));
+                const float fall = m[n][r] - ref;
+                x0 -= ref, x1 -= ref;
+                sum[n][r] = sum[n][r] * exp2_fast(fall) + (exp2_fast(x0) + exp2_fast(x1));
                 m[n][r] = m1;
-                const float v1 = fmaxf(mv[n][r], top + lv), vref = v1 == -CUDART_INF_F ? 0.f : v1;
-                turn[r] = exp2_fast(mv[n][r] - vref);
-                moved |= v1 != mv[n][r];
+                const float v0 = mv[n][r] + fall, v1 = fmaxf(fmaxf(v0, (top - ref) + lv), kLeastUnit);
+                turn[r] = exp2_fast(v0 - v1);
+                moved |= v1 != v0;
                 mv[n][r] = v1;
-                p[r][0] = exp2_fast(x0 + (lv - vref));
-                p[r][1] = exp2_fast(x1 + (lv - vref));
+                const float up = (lv - v1) + kWeightExponent;
+                p[r][0] = exp2_fast(x0 + up);
+                p[r][1] = exp2_fast(x1 + up);
             }
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -523,7 +533,7 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
     cp_wait<0>();
     __syncthreads();
 
-    // join the CTA's warps.  A warp's O moves from units of 2^mv to units of 2^m.
+    // join the CTA's warps.  A warp's O moves from units of 2^(m + mv - 15) to units of 2^m.
     float *mine_o = reinterpret_cast<float *>(ring);
     float *mine_m = mine_o + L::kRows * DP;
 #pragma unroll
@@ -533,7 +543,9 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
             float l = sum[n][r];
 #pragma unroll
             for (int w = 4; w <= 16; w <<= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-            const float unit = mv[n][r] == -CUDART_INF_F ? 0.f : exp2_fast(mv[n][r] - m[n][r]);
+            const float unit = exp2_fast(mv[n][r]);
+#pragma unroll
+            for (int d = 0; d < DP / 16; ++d) o[n][d][r] *= kWeightDown, o[n][d][2 + r] *= kWeightDown;
             const int row = 8 * n + 2 * t + r;
             if (g == 0) {
                 mine_m[row] = m[n][r];

@@ -540,3 +540,69 @@ def test_refusals(calls):
     assert bool((cache.attention(x, no_blocks, lens) == 0).all())
     assert bool((cache.gather(no_blocks, lens, 5)[0] == 0).all())
     cache.append(x, x, no_blocks, lens)
+
+
+# ------------------------------------------------------------------------------------ small weights, limits
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [14, 20, 24, 27])
+@pytest.mark.parametrize("n", [4000, 40000])
+def test_light_tails_beside_dominating_tokens(dtype, bits, n):
+    """Tokens whose weights are 2^-bits of the largest ones', where the largest belong to values of zero: what is
+    left is the tail's weighted sum.
+
+    Tolerance: as for attention above, but what a weight loses below float16's normal range is 2^-40 of the
+    largest p * step at most: weights are scaled by 2^15 before they are rounded, an absolute step there is 2^-24, half of it
+    the rounding."""
+    page, dim, group = 16, 64, 2
+    pages = n // page + 3
+    cache = make_cache(pages, 1, page, dim, seed=bits)
+    table = make_table([n], page, pages)
+    cache.value.abs_().clamp_(min=64)
+    cache.value_scale.mul_(100.0)
+    cache.key.zero_()
+    # a dominating token at the start of four tiles of every sixteen, so that every warp meets some
+    at = torch.arange(n, device="cuda")
+    first = at[(at % 16 == 0) & ((at // 16) % 16 < 4)]
+    where, row = table[0, first // page].long(), first % page
+    cache.key[where, 0, row, 0] = LEVELS
+    cache.value[where, 0, row] = 0
+    cache.key_scale.fill_(1 / LEVELS)
+    q = torch.zeros(1, 1, group, dim, device="cuda")
+    q[..., 0] = torch.tensor([bits, bits + 0.5], device="cuda") * 0.6931471805599453
+    q[..., 1] = 1.0
+    q = q.to(dtype)
+    got = cache.attention(q, table, ints([n]), scale=1.0)[0, 0].double()
+    k, _, _ = values_of(cache, "key", table, 0, n)
+    v, _, step = values_of(cache, "value", table, 0, n)
+    score = q[0, 0].double() @ k[0].T
+    off = (q[0, 0].double().abs() @ k[0].abs().T).amax(-1, keepdim=True) * (dim / 16 + 8) * 2.0**-23
+    p = torch.softmax(score, -1)
+    want = p @ v[0]
+    half = torch.finfo(dtype).eps / 2
+    small = 2.0**-21 if dtype == torch.float32 else 2.0**-11
+    bound = half * want.abs() + (p @ v[0].abs()) * (2 * off + small + 2.0**-17) + n * 2.0**-40 * (p * step).amax(-1, keepdim=True) * LEVELS
+    if dtype == torch.float16:
+        bound = bound + 2.0**-25
+    err = (got - want).abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.5, 2.0**22])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_scores_of_any_size_stay_finite(dtype, scale):
+    """A softmax scale of zero or below, and scores so large that float32 steps are whole powers of two between
+    them: a weighted mean of values whatever the scores."""
+    cache = make_cache(30, 1, 16, 64, seed=2)
+    table = make_table([400], 16, 30)
+    q = torch.randn(1, 1, 4, 64, generator=torch.Generator().manual_seed(5)).to(dtype).cuda() * 3
+    got, lse = cache.attention(q, table, ints([400]), scale=scale, return_lse=True)
+    assert bool(torch.isfinite(got).all()) and bool(torch.isfinite(lse).all())
+    if abs(scale) < 1:
+        check_attention(cache, q, table, [400], None, scale=scale)
+    else:  # one token is all there is
+        k, _, _ = values_of(cache, "key", table, 0, 400)
+        v, _, _ = values_of(cache, "value", table, 0, 400)
+        assert bool((got[0, 0].double() <= v.amax() * 1.01).all())
+    # all but one page of values that are zero: what is left is far below the largest score, or not
+    cache.value_scale[table[0, 1:].long()] = 0.0
+    assert bool(torch.isfinite(cache.attention(q, table, ints([400]), scale=scale)).all())
