@@ -181,16 +181,17 @@ template <typename E> __device__ __forceinline__ void store4(E *dst, const float
     }
 }
 
-// What a sequence's row block sees: tokens [lo, hi)
+// What a sequence's row block sees: tokens [lo, hi).  Positions count all of the context, tokens are those that the
+// table has room for.
 struct Span {
     int lo, hi;
 };
-__device__ __forceinline__ Span span_of(const AttnArgs &a, int ctx, int len, int first_token, int last_token) {
+__device__ __forceinline__ Span span_of(const AttnArgs &a, int ctx, int cap, int len, int first_token, int last_token) {
     Span s;
     const int base = ctx - len;  // position of the first query token; negative if there are more than the context
     s.hi = a.causal ? min(ctx, base + last_token + 1) : ctx;
     s.lo = a.window > 0 ? max(0, base + first_token - a.window + 1) : 0;
-    s.hi = max(s.hi, 0);
+    s.hi = max(min(s.hi, cap), 0);
     s.lo = min(s.lo, s.hi);
     return s;
 }
@@ -255,12 +256,12 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
     }
 
     const int cap = (int)min((long long)a.table_width * a.page, 0x7fffffffll);
-    const int ctx = min(max(a.context[s], 0), cap);
+    const int ctx = max(a.context[s], 0);
     const int len = a.qlens ? min(max(a.qlens[s], 0), a.tokens) : a.tokens;
     const int live = min(max(len * a.group - row0, 0), L::kRows);  // rows of this block with a query
     const int first_token = row0 / a.group, last_token = (row0 + live - 1) / a.group;
     Span span = {0, 0};
-    if (live > 0) span = span_of(a, ctx, len, first_token, last_token);
+    if (live > 0) span = span_of(a, ctx, cap, len, first_token, last_token);
     int from = span.lo, to = span.hi, count = 1;  // pieces of this row block
     if (a.part) {
         const int n = piece_tokens(a, lane);
@@ -374,7 +375,7 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
             score_scale[n][i] = __shfl_sync(0xffffffffu, down, (2 * t + i) * 4);
             const int row = 8 * n + 2 * t + i;
             const int tok = row < live ? (row0 + row) / a.group : first_token;
-            const Span sp = live > 0 ? span_of(a, ctx, len, tok, tok) : Span{0, 0};
+            const Span sp = live > 0 ? span_of(a, ctx, cap, len, tok, tok) : Span{0, 0};
             lo_row[n][i] = sp.lo;
             hi_row[n][i] = sp.hi;
             max_lo = max(max_lo, sp.lo);

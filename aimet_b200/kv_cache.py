@@ -244,7 +244,8 @@ class Int8KVCache:
         cache's (consecutive query heads share a cache head); ``context_lens``: int32 tokens in the cache,
         the newest included (append first); ``query_lens``: int32 tokens of ``query`` that are real
         (default: all).  Query ``i`` stands at position ``context_lens - query_lens + i`` and sees positions
-        up to its own (``causal``) and after its own minus ``window``; ``scale`` defaults to
+        up to its own (``causal``) and after its own minus ``window``, as far as they have a page (positions behind
+        the table's end have none); ``scale`` defaults to
         ``head_dim ** -0.5``.  Scores, softmax and sums are float32.
 
         Returns ``[sequences, tokens, heads, head_dim]`` in ``query.dtype``; queries that see nothing, and

@@ -606,3 +606,18 @@ def test_scores_of_any_size_stay_finite(dtype, scale):
     # all but one page of values that are zero: what is left is far below the largest score, or not
     cache.value_scale[table[0, 1:].long()] = 0.0
     assert bool(torch.isfinite(cache.attention(q, table, ints([400]), scale=scale)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page,width,context,tokens,window,causal", [
+    (16, 6, [98, 96, 200], 5, None, True), (16, 6, [98, 110, 400], 5, 40, True), (32, 3, [97, 100, 99], 4, 7, False),
+    (16, 700, [11210, 11200, 30000], 20, 300, True), (16, 700, [11205], 8, None, True),
+])
+def test_contexts_that_reach_behind_the_table(dtype, page, width, context, tokens, window, causal):
+    """Tokens behind the table's last block have no page: masked, and positions count them all the same."""
+    pages = len(context) * width + 2
+    cache = make_cache(pages, 1, page, 64, seed=width)
+    table = make_table([width * page] * len(context), page, pages)
+    q = torch.randn(len(context), tokens, 3, 64, generator=torch.Generator().manual_seed(6)).to(dtype).cuda()
+    check_attention(cache, q, table, context, None, window=window, causal=causal)
+    check_attention(cache, q, table, context, [tokens - 2] * len(context), window=window, causal=causal)
