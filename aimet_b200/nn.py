@@ -128,8 +128,8 @@ def compute_encodings(model: nn.Module, group=None):
                     quantizers.append(q)
         # the weights do not change while the calibration data runs through: each is quantized once
         # here instead of on every forward inside the context (no-grad forwards only)
-        _hold_quantized_weights(layers)
         try:
+            _hold_quantized_weights(layers)
             yield
         finally:
             for layer in layers:
@@ -217,17 +217,17 @@ def precomputed(model: nn.Module, packed: bool = False):
                   if q is not None and q.is_initialized()]
         for q, enc in zip(frozen, derive_encodings(frozen)):
             stack.enter_context(q._set_encodings(enc))  # pylint: disable=protected-access
-        for layer in layers:
-            qw = layer.param_quantizers["weight"]
-            if packed and _packable(layer):
-                try:
-                    layer.__dict__["_packed_weight"] = PackedInt4Weight.from_quantizer(layer.layer.weight, qw)
-                    continue
-                except NotImplementedError:
-                    pass
-            if qw is not None and qw.is_initialized():
-                layer.__dict__["_held_weight"] = qw(layer.layer.weight).detach()
         try:
+            for layer in layers:
+                qw = layer.param_quantizers["weight"]
+                if packed and _packable(layer):
+                    try:
+                        layer.__dict__["_packed_weight"] = PackedInt4Weight.from_quantizer(layer.layer.weight, qw)
+                        continue
+                    except NotImplementedError:
+                        pass
+                if qw is not None and qw.is_initialized():
+                    layer.__dict__["_held_weight"] = qw(layer.layer.weight).detach()
             yield model
         finally:
             for layer in layers:

@@ -478,3 +478,45 @@ def test_packed_weights_against_the_weights_held_otherwise(dtype, tokens, grid):
                 bound = bound + 2.0**-23 * (x.double().abs() @ w.abs().T)
             assert bool(((got.double() - want.double()).abs() <= bound).all())
             x = want
+
+
+def test_a_context_that_fails_on_entry_leaves_no_frozen_weight(monkeypatch):
+    """Packing, or quantizing, the second layer's weight raises: the first layer keeps nothing, and a weight that is
+    edited afterwards counts."""
+    from aimet_b200 import int4
+    from aimet_b200 import nn as qnn
+    from aimet_b200.quantizer import QuantizeDequantize
+
+    model = layers_of(torch.float32)
+    x = torch.randn(4, 64, device="cuda")
+    made = int4.PackedInt4Weight.from_quantizer.__func__
+
+    def breaks(cls, weight, quantizer):
+        if weight is model[1].layer.weight:
+            raise MemoryError("no room")
+        return made(cls, weight, quantizer)
+
+    with monkeypatch.context() as patch:
+        patch.setattr(int4.PackedInt4Weight, "from_quantizer", classmethod(breaks))
+        with pytest.raises(MemoryError), qnn.precomputed(model, packed=True):
+            pass
+
+    def quantizing(self, t):
+        if t.shape == model[1].layer.weight.shape:
+            raise MemoryError("no room")
+        return plain(self, t)
+
+    plain = QuantizeDequantize.forward
+    for context in (qnn.precomputed, qnn.compute_encodings):
+        with monkeypatch.context() as patch:
+            patch.setattr(QuantizeDequantize, "forward", quantizing)
+            for layer in model:
+                layer.param_quantizers["weight"].allow_overwrite(False)
+            with pytest.raises(MemoryError), context(model):
+                pass
+    for layer in model:
+        assert "_packed_weight" not in layer.__dict__ and "_held_weight" not in layer.__dict__
+    with torch.no_grad():
+        before = model(x)
+        model[0].layer.weight.data.mul_(-1)
+        assert not torch.equal(before, model(x))
