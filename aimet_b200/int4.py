@@ -202,11 +202,14 @@ class PackedInt4Weight:
     def from_encoding(cls, weight: torch.Tensor, encoding) -> "PackedInt4Weight":
         """Quantize ``weight`` ``[out_features, in_features]`` with a 4-bit ``AffineEncoding`` (per tensor, per
         output channel, or blockwise along the input channels) and pack the codes: the ones that
-        ``quantize_dequantize`` simulates when no gradient is wanted."""
+        ``quantize_dequantize`` simulates when no gradient is wanted.  What 4 bits cannot hold (a wider grid, a
+        scale per input channel, NaN) raises ``NotImplementedError``."""
         if weight.dim() != 2:
             raise NotImplementedError(f"weights of linear layers are packed, got shape {tuple(weight.shape)}")
         if encoding.qmax - encoding.qmin > 15:
             raise NotImplementedError(f"a grid of [{encoding.qmin}, {encoding.qmax}] does not fit 4 bits")
+        if not -128 <= encoding.qmin <= 112:
+            raise NotImplementedError(f"codes of [{encoding.qmin}, {encoding.qmax}] do not fit signed bytes")
         if encoding.zero_point_shift:
             raise NotImplementedError("a grid with a zero-point shift cannot be packed")
         n, k = weight.shape
@@ -215,6 +218,8 @@ class PackedInt4Weight:
             if scale.dim() > 2:
                 raise NotImplementedError(f"scales of shape {tuple(scale.shape)} for a linear layer's weight")
             codes = _simulated_codes(weight.detach(), encoding)
+            if not bool(torch.isfinite(codes).all()):
+                raise NotImplementedError("a weight or scale that is not a number has no codes")
 
             def per_channel(p):  # [out or 1, blocks] -> [out, blocks]
                 p = p.detach().to(torch.float32).reshape((1,) * (2 - p.dim()) + tuple(p.shape))

@@ -520,3 +520,22 @@ def test_a_context_that_fails_on_entry_leaves_no_frozen_weight(monkeypatch):
         before = model(x)
         model[0].layer.weight.data.mul_(-1)
         assert not torch.equal(before, model(x))
+
+
+def test_weights_without_codes_are_held_as_they_are():
+    """A weight that holds NaN, or an infinity, runs packed as it runs held."""
+    from aimet_b200 import nn as qnn
+
+    for grid in ("per_channel", "blockwise"):
+        for bad in (float("nan"), float("inf")):
+            model = layers_of(torch.float32, grid=grid)
+            model[1].layer.weight.data[3, 5] = bad
+            x = torch.randn(4, 64, device="cuda")
+            with torch.no_grad():
+                with qnn.precomputed(model):
+                    want = model[1](model[0](x))
+                with qnn.precomputed(model, packed=True):
+                    assert "_packed_weight" in model[0].__dict__
+                    got = model[1](model[0](x))
+            assert torch.equal(torch.isnan(got), torch.isnan(want))
+            assert bool(((got - want).abs().nan_to_num() <= 1e-4 * want.abs().nan_to_num().amax()).all())
