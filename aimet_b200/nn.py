@@ -54,7 +54,12 @@ class QuantizedLayer(nn.Module):
             x = qi(x)
         packed = self.__dict__.get("_packed_weight")
         if packed is not None and not torch.is_grad_enabled() and getattr(qw, "_observer_hook", None) is None:
-            out = linear_int4(x, packed, self.layer.bias)
+            bias = self.layer.bias
+            if torch.is_autocast_enabled("cuda"):  # the types that autocast gives the plain product
+                dtype = torch.get_autocast_dtype("cuda")
+                x = x.to(dtype) if x.is_floating_point() and x.dtype != torch.float64 else x
+                bias = bias if bias is None else bias.to(dtype)
+            out = linear_int4(x, packed, bias)
             return out if qo is None else qo(out)
         w = self.layer.weight if qw is None else self._quantized_weight(qw)
         if isinstance(self.layer, nn.Conv2d):
@@ -206,8 +211,9 @@ def precomputed(model: nn.Module, packed: bool = False):
 
     ``packed``: Linear layers with weights of at most 4 bits hold their codes packed
     (:class:`aimet_b200.int4.PackedInt4Weight`) instead of the quantize-dequantized weight, a quarter of
-    its bytes in 16 bits, and multiply with them directly in no-grad forwards.  Grids that cannot be
-    packed, and layers of other kinds, are held as without ``packed``."""
+    its bytes in 16 bits, and multiply with them directly in no-grad forwards, in the types that autocast
+    asks for where it is on.  Grids that cannot be packed, and layers of other kinds, are held as without
+    ``packed``."""
     from .quantizer import derive_encodings
 
     with contextlib.ExitStack() as stack, torch.no_grad():

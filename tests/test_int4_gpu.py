@@ -539,3 +539,26 @@ def test_weights_without_codes_are_held_as_they_are():
                     got = model[1](model[0](x))
             assert torch.equal(torch.isnan(got), torch.isnan(want))
             assert bool(((got - want).abs().nan_to_num() <= 1e-4 * want.abs().nan_to_num().amax()).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens", [1, 7, 40])
+def test_packed_weights_under_autocast(dtype, tokens):
+    """Autocast decides the types of a packed layer's product as it does of the plain one: activations of any type
+    it casts, a float32 bias among them."""
+    from aimet_b200 import nn as qnn
+
+    model = layers_of(torch.float32)
+    layer = model[0]
+    for given in (torch.float32, dtype):
+        x = torch.randn(tokens, 64, device="cuda").to(given)
+        with torch.no_grad(), torch.autocast("cuda", dtype=dtype):
+            with qnn.precomputed(model):
+                want, w = layer(x), layer._held_weight.double()
+                deep = model(x)
+            with qnn.precomputed(model, packed=True):
+                got = layer(x)
+                assert model(x).dtype == deep.dtype == dtype
+        assert got.dtype == want.dtype == dtype
+        bound = linear_bound(x.to(dtype), w, layer.layer.bias.to(dtype), dtype, 2)
+        assert bool(((got.double() - want.double()).abs() <= bound).all())
