@@ -10,6 +10,7 @@ import os
 from typing import Sequence
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libaimet_b200.so")
@@ -275,6 +276,13 @@ class _Scratch:
 
 
 scratch = _Scratch()
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of the tensors carries a forward-mode derivative, which operators without one would drop (it is
+    followed with gradients switched off too)."""
+    return (_forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()  # pylint: disable=protected-access
+            and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors))
 
 
 def _load_calls():

@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -26,12 +27,13 @@ decltype(&aimet_b200_kv_attention_scratch_bytes) g_scratch;
 int code_of(at::ScalarType t) {
     return t == at::kFloat ? AB_F32 : t == at::kHalf ? AB_F16 : t == at::kBFloat16 ? AB_BF16 : -1;
 }
-// a plain tensor on the current device `index` that autograd does not have to follow; else nullptr
+// a plain tensor on the current device `index` that autograd does not have to follow, backwards or forwards; else nullptr
 const at::Tensor *plain(PyObject *o, int64_t index) {
     if (!THPVariable_CheckExact(o)) return nullptr;
     const at::Tensor &t = THPVariable_Unpack(o);
     if (!t.is_cuda() || t.get_device() != index) return nullptr;
     if (t.requires_grad() && c10::GradMode::is_enabled()) return nullptr;
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined()) return nullptr;
     return &t;
 }
 const at::Tensor *lengths(PyObject *o, int64_t index, int64_t n) {

@@ -252,8 +252,8 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
     float32, float16 or bfloat16 activations; sums in float32, one rounding to ``input.dtype``.  A few
     tokens, and float32 always, multiply the integer codes exactly; many tokens multiply weights that are
     rounded to the 16-bit type once, as a simulated 16-bit model's are.  Rows of up to 37120 input features in
-    float32 and 111360 in 16 bits.  For inference: an input or bias that needs a gradient is refused (train
-    through the quantizer instead).
+    float32 and 111360 in 16 bits.  For inference: an input or bias that needs a gradient, or carries a
+    forward-mode derivative, is refused (train through the quantizer instead).
     """
     if _calls is not None:
         out = _calls.linear(input, bias, weight._address, weight._index, weight._status)  # pylint: disable=protected-access
@@ -265,6 +265,8 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
         plan = _plan_linear(signature, input, weight)
     if torch.is_grad_enabled() and (input.requires_grad or (bias is not None and bias.requires_grad)):
         raise RuntimeError("linear_int4 has no backward pass: call it under torch.no_grad(), or train through the weight's quantizer")
+    if _lib.has_tangent(input, bias):
+        raise RuntimeError("linear_int4 has no forward-mode derivative: train through the weight's quantizer")
     code, tokens, pitch, out_shape, direct, watched = plan
     if bias is not None:
         if bias.dtype != input.dtype or bias.get_device() != input.get_device() or bias.shape != weight._bias_shape:  # pylint: disable=protected-access

@@ -6,7 +6,8 @@ into it, :meth:`Int8KVCache.attention` attends over it reading one byte per elem
 :meth:`Int8KVCache.gather` reads tokens back as values.  Token ``j`` of a sequence lies in row
 ``j % page_size`` of page ``block_table[sequence, j // page_size]``; which pages belong to whom is the
 caller's, lengths and tables stay on the device, nothing waits for the host, so a decode step can be
-captured into a CUDA graph.  Inference only: inputs that need a gradient are refused.
+captured into a CUDA graph.  Inference only: inputs that need a gradient, or carry a forward-mode
+derivative, are refused.
 """
 
 from __future__ import annotations
@@ -165,6 +166,8 @@ class Int8KVCache:
         plan = self._plans.get(signature) or self._plan_append(signature, key, value, block_table, context_lens, new_lens)
         if torch.is_grad_enabled() and (key.requires_grad or value.requires_grad):
             raise RuntimeError("append has no backward pass: call it under torch.no_grad()")
+        if _lib.has_tangent(key, value):
+            raise RuntimeError("append has no forward-mode derivative")
         code, key_strides, value_strides, dense = plan
         if not dense:
             block_table, context_lens, new_lens = self._dense(block_table, context_lens, new_lens)
@@ -266,6 +269,8 @@ class Int8KVCache:
         plan = self._plans.get(signature) or self._plan_attention(signature, query, block_table, context_lens, query_lens, window)
         if torch.is_grad_enabled() and query.requires_grad:
             raise RuntimeError("attention over the cache has no backward pass: call it under torch.no_grad()")
+        if _lib.has_tangent(query):
+            raise RuntimeError("attention over the cache has no forward-mode derivative")
         code, strides, group, need, dense = plan
         if not dense:
             block_table, context_lens, query_lens = self._dense(block_table, context_lens, query_lens)

@@ -17,6 +17,7 @@ from typing import Callable, Iterable, Optional
 import torch
 from torch import nn
 
+from ._lib import has_tangent
 from .encoding_analyzer import MinMaxEncodingAnalyzer
 from .int4 import MOST_FEATURES, PackedInt4Weight, linear_int4
 from .quantizer import QuantizeDequantize
@@ -53,8 +54,9 @@ class QuantizedLayer(nn.Module):
         if qi is not None:
             x = qi(x)
         packed = self.__dict__.get("_packed_weight")
-        if packed is not None and not torch.is_grad_enabled() and getattr(qw, "_observer_hook", None) is None:
-            bias = self.layer.bias
+        bias = self.layer.bias
+        if (packed is not None and not torch.is_grad_enabled() and getattr(qw, "_observer_hook", None) is None
+                and not has_tangent(x, bias)):
             if torch.is_autocast_enabled("cuda"):  # the types that autocast gives the plain product
                 dtype = torch.get_autocast_dtype("cuda")
                 x = x.to(dtype) if x.is_floating_point() and x.dtype != torch.float64 else x

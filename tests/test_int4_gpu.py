@@ -562,3 +562,32 @@ def test_packed_weights_under_autocast(dtype, tokens):
         assert got.dtype == want.dtype == dtype
         bound = linear_bound(x.to(dtype), w, layer.layer.bias.to(dtype), dtype, 2)
         assert bool(((got.double() - want.double()).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("off", [False, True])
+def test_forward_mode_derivatives_are_refused(calls, off):
+    """A tangent would be lost: refused, with gradients off too; a packed layer multiplies with the simulated weight."""
+    import torch.autograd.forward_ad as fwad
+
+    from aimet_b200 import nn as qnn
+    from aimet_b200.int4 import linear_int4
+
+    parts = make(48, 64, 64, "sym")
+    p = packed_of(*parts)
+    x, bias = torch.randn(3, 64, device="cuda"), torch.randn(48, device="cuda")
+    model = layers_of(torch.float32)
+    with torch.set_grad_enabled(not off), fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            linear_int4(dual, p)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            linear_int4(x, p, fwad.make_dual(bias, torch.ones_like(bias)))
+        assert linear_int4(x, p, bias).shape == (3, 48)
+        with fwad._set_fwd_grad_enabled(False):
+            assert torch.equal(linear_int4(dual, p), linear_int4(x, p))
+        with torch.no_grad():
+            with qnn.precomputed(model):
+                want = fwad.unpack_dual(model(dual)).tangent
+            with qnn.precomputed(model, packed=True):
+                got = fwad.unpack_dual(model(dual)).tangent
+        assert want is not None and torch.equal(got, want)

@@ -621,3 +621,21 @@ def test_contexts_that_reach_behind_the_table(dtype, page, width, context, token
     q = torch.randn(len(context), tokens, 3, 64, generator=torch.Generator().manual_seed(6)).to(dtype).cuda()
     check_attention(cache, q, table, context, None, window=window, causal=causal)
     check_attention(cache, q, table, context, [tokens - 2] * len(context), window=window, causal=causal)
+
+
+@pytest.mark.parametrize("off", [False, True])
+def test_forward_mode_derivatives_are_refused(calls, off):
+    import torch.autograd.forward_ad as fwad
+
+    cache = make_cache(4, 2, 16, 32)
+    table, lens = ints([[0, 1]]), ints([3])
+    x = torch.randn(1, 1, 2, 32, device="cuda")
+    with torch.set_grad_enabled(not off), fwad.dual_level():
+        dual = fwad.make_dual(x, torch.ones_like(x))
+        for key, value in ((dual, x), (x, dual)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                cache.append(key, value, table, lens)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            cache.attention(dual, table, lens)
+        cache.append(x, x, table, lens)
+        assert cache.attention(x, table, lens).shape == x.shape
