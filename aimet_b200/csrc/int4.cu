@@ -264,7 +264,8 @@ __global__ void __launch_bounds__(kMvWarps * 32, 2) k_matvec(Int4View w, const E
                     if (a < hi && b > lo && a < b) v += part[q][a < lo ? 1 : 0][at];
                 }
             }
-            v *= w.row_scale[n] * (1.f / Pair16<H>::kUnit);
+            const RowFactor f = row_factor<H>(w.row_scale[n]);
+            v = v * f.unit * f.scale;
             if (bias) v += to_f32(bias[n]);
             y[(int64_t)(m0 + m) * ldy + n] = Cvt<float, E>::store(v);
         }

@@ -85,6 +85,16 @@ template <> struct Pair16<__half> {
 template <typename H> __device__ __forceinline__ uint32_t zero_pair(float z) {
     return Pair16<H>::both(-(Pair16<H>::kBase + z) * Pair16<H>::kUnit);
 }
+// What a channel's sum of code * kUnit * x is multiplied by: first `unit`, then `scale`; together row_scale / kUnit, which
+// by itself may be no float32 number although the result is one.
+struct RowFactor {
+    float unit, scale;
+};
+template <typename H> __device__ __forceinline__ RowFactor row_factor(float row_scale) {
+    constexpr float kUp = 1.f / Pair16<H>::kUnit;
+    if constexpr (kUp == 1.f) return {1.f, row_scale};
+    return fabsf(row_scale) < 1.f ? RowFactor{1.f, row_scale * kUp} : RowFactor{kUp, row_scale};
+}
 // the codes of pair p (0..3) of a word as two 16-bit floats, (u - z) * kUnit
 template <typename H> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int p, uint32_t zero2) {
     uint32_t v;

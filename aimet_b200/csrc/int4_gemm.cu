@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
                     for (int j = 0; j < 16; ++j) sums[(c + j) * kChannels] = __uint_as_float(r[j]);
                 }
             } else {
-                const float f = live ? a.w.row_scale[n] * (1.f / Pair16<E>::kUnit) : 0.f;
+                const RowFactor f = row_factor<E>(live ? a.w.row_scale[n] : 0.f);
                 const float b = live && a.bias ? to_f32(static_cast<const E *>(a.bias)[n]) : 0.f;
                 const int m0 = tile / a.n_ct * a.bn;
                 E *y = static_cast<E *>(a.y) + (int64_t)m0 * a.ldy + n;
@@ -336,13 +336,13 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
                     tmem_ld16(t0 + c + 16, rb);
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
-                        if (live && c + j < left) y[(int64_t)(c + j) * a.ldy] = Cvt<float, E>::store(fmaf(__uint_as_float(ra[j]), f, b));
+                        if (live && c + j < left) y[(int64_t)(c + j) * a.ldy] = Cvt<float, E>::store(fmaf(__uint_as_float(ra[j]) * f.unit, f.scale, b));
                     __syncwarp();  // (reading tensor memory is a warp's lanes together, after stores that some lanes skip)
                     tmem_ld_wait();
                     if (c + 32 < a.bn) tmem_ld16(t0 + c + 32, ra);
 #pragma unroll
                     for (int j = 0; j < 16; ++j)
-                        if (live && c + 16 + j < left) y[(int64_t)(c + 16 + j) * a.ldy] = Cvt<float, E>::store(fmaf(__uint_as_float(rb[j]), f, b));
+                        if (live && c + 16 + j < left) y[(int64_t)(c + 16 + j) * a.ldy] = Cvt<float, E>::store(fmaf(__uint_as_float(rb[j]) * f.unit, f.scale, b));
                     __syncwarp();
                 }
             }
@@ -372,7 +372,8 @@ __global__ void __launch_bounds__(kThreads4, 1) k_int4_gemm(const __grid_constan
                 asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(there) : "memory");
                 v += f;
             }
-            v *= a.w.row_scale[n0 + ch] * (1.f / Pair16<E>::kUnit);
+            const RowFactor f = row_factor<E>(a.w.row_scale[n0 + ch]);
+            v = v * f.unit * f.scale;
             if (a.bias) v += to_f32(static_cast<const E *>(a.bias)[n0 + ch]);
             static_cast<E *>(a.y)[(int64_t)(m0 + col) * a.ldy + n0 + ch] = Cvt<float, E>::store(v);
         }

@@ -591,3 +591,18 @@ def test_forward_mode_derivatives_are_refused(calls, off):
             with qnn.precomputed(model, packed=True):
                 got = fwad.unpack_dual(model(dual)).tangent
         assert want is not None and torch.equal(got, want)
+
+
+@pytest.mark.parametrize("grid", ["sym", "lpbq"])
+@pytest.mark.parametrize("tokens", [1, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_scales_near_the_end_of_the_range(dtype, tokens, grid):
+    """Scales of 2^120 and more beside small activations: the product is a number of the type."""
+    from aimet_b200.int4 import linear_int4
+
+    codes, scale, offset, qmin, int_scale = make(40, 128, 64, grid)
+    scale = scale * 2.0**126
+    x = (torch.randn(tokens, 128, generator=torch.Generator().manual_seed(3)) * 2.0**-60).to(dtype).cuda()
+    w = dequantized(codes, scale, offset, int_scale)
+    got = linear_int4(x, packed_of(codes, scale, offset, qmin, int_scale))
+    assert_close(got, x, w, weight_in_16=tokens > 8 and dtype != torch.float32)
