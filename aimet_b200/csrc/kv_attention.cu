@@ -73,6 +73,7 @@ struct AttnArgs {
     int64_t table_stride;
     uint32_t page_magic;  // tile / (page / kTokens) == umulhi(tile, page_magic) (tiles below 2^26, at most 64 in a page); 0: one tile in a page
     int table_width, seqs, tokens, group, row_blocks, pieces;
+    int first_block, blocks;  // row blocks of this launch
     int causal, window, vec;
     int target;        // CTAs per head and row block that fill the machine
     float scale_log2;  // softmax scale * log2(e)
@@ -239,7 +240,7 @@ template <typename E, int DP, int NQ, bool FULL> __global__ void __launch_bounds
     constexpr int QS = F32 ? 2 : 1;   // float16 terms of q and of the weights
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int piece = blockIdx.x, h = blockIdx.y / a.row_blocks, rb = blockIdx.y % a.row_blocks, s = blockIdx.z;
+    const int piece = blockIdx.x, h = blockIdx.y / a.blocks, rb = a.first_block + blockIdx.y % a.blocks, s = blockIdx.z;
     const int rows = a.tokens * a.group;  // of the output
     const int row0 = rb * L::kRows;
     pdl_prologue();
@@ -728,17 +729,16 @@ int check_call(const ab_kv_cache *c, int64_t seqs, int64_t tokens, int64_t group
         return fail(AB_ERR_INVALID, "seqs=%lld tokens=%lld group=%lld table_width=%lld", (long long)seqs, (long long)tokens, (long long)group,
                     (long long)table_width);
     if (c->num_heads < 1 || c->num_heads > 1024) return fail(AB_ERR_INVALID, "num_heads=%d", c->num_heads);
-    if (seqs * tokens * group * c->num_heads > 0x7fffffff || (int64_t)c->num_heads * div_up(tokens * group, 16) > 65535)
+    if (seqs * tokens * group * c->num_heads > 0x7fffffff || (int64_t)c->num_heads * div_up(tokens * group, 16) >= (1 << 20))
         return fail(AB_ERR_UNSUPPORTED, "%lld query rows of %d heads in one call", (long long)(tokens * group), c->num_heads);
     return AB_OK;
 }
 
-template <typename E, int DP, int NQ, bool FULL> int launch_as(const AttnArgs &a, cudaStream_t st) {
+template <typename E, int DP, int NQ, bool FULL> int launch_as(AttnArgs a, cudaStream_t st) {
     using L = Layout<E, DP, NQ>;
     const int rc = opt_in_smem<k_kv_attention<E, DP, NQ, FULL>>(L::kSmem);
     if (rc != AB_OK) return rc;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.pieces, (unsigned)(a.heads * a.row_blocks), (unsigned)a.seqs);
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = L::kSmem;
     cfg.stream = st;
@@ -750,8 +750,14 @@ template <typename E, int DP, int NQ, bool FULL> int launch_as(const AttnArgs &a
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = !a.part && a.pieces > 1 ? 2 : 1;
-    AB_CUDA_OK(cudaLaunchKernelEx(&cfg, k_kv_attention<E, DP, NQ, FULL>, a));
-    AB_LAUNCH_OK();
+    // what the grid's second dim does not hold (prompts of many heads) takes further launches
+    const int most = 65535 / a.heads;
+    for (a.first_block = 0; a.first_block < a.row_blocks; a.first_block += most) {
+        a.blocks = std::min(most, a.row_blocks - a.first_block);
+        cfg.gridDim = dim3((unsigned)a.pieces, (unsigned)(a.heads * a.blocks), (unsigned)a.seqs);
+        AB_CUDA_OK(cudaLaunchKernelEx(&cfg, k_kv_attention<E, DP, NQ, FULL>, a));
+        AB_LAUNCH_OK();
+    }
     if (a.part) {  // (check_call bounds the rows)
         const int64_t rows = (int64_t)a.seqs * a.tokens * a.heads * a.group;
         AB_CUDA_OK(launch_pdl(k_kv_join<E>, dim3((unsigned)rows), dim3(kJoinWarps * 32), 0, st, a, L::kRows));

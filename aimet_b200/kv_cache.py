@@ -254,7 +254,8 @@ class Int8KVCache:
         Returns ``[sequences, tokens, heads, head_dim]`` in ``query.dtype``; queries that see nothing, and
         those behind ``query_lens``, give zeros.  With ``return_lse`` also the logarithm of each query's
         softmax sum, float32 ``[sequences, tokens, heads]`` (-inf where it sees nothing), by which results
-        over parts of a context can be joined.
+        over parts of a context can be joined.  In one call up to 65535 sequences, and fewer than 2^20 sixteens of
+        query rows (tokens times query heads for each of the cache's) over all of the cache's heads.
         """
         scale = self._scale if scale is None else float(scale)
         if _calls is not None and (window is None or window >= 1):

@@ -462,8 +462,10 @@ int aimet_b200_kv_gather(const ab_kv_cache *cache, void *key, void *value, int64
  * j < context_lens[s] (which counts the newest tokens); query [seqs][tokens][num_heads * group][head_dim],
  * head h reads head h / group of the cache.  Query i < query_lens[s] (NULL: all) stands at position
  * p = context_lens[s] - query_lens[s] + i; causal != 0: j <= p; window > 0: j > p - window.  Positions that
- * the table has no room for are masked as those without a page are.  Rows that see nothing, and rows behind query_lens[s], are zero.  lse (float32 [seqs][tokens][num_heads * group], may be
- * NULL): log of the sum of exp(score), -infinity for those rows. */
+ * the table has no room for are masked as those without a page are.  Rows that see nothing, and rows behind
+ * query_lens[s], are zero.  lse (float32 [seqs][tokens][num_heads * group], may be NULL): log of the sum of
+ * exp(score), -infinity for those rows.  Up to 65535 sequences, and num_heads * ceil(tokens * group / 16) below
+ * 2^20. */
 int64_t aimet_b200_kv_attention_scratch_bytes(const ab_kv_cache *cache, int64_t seqs, int64_t tokens, int64_t group,
                                               int64_t table_width, int io_dtype);
 int aimet_b200_kv_attention(const ab_kv_cache *cache, const void *query, const int64_t *query_strides, void *out,

@@ -639,3 +639,25 @@ def test_forward_mode_derivatives_are_refused(calls, off):
             cache.attention(dual, table, lens)
         cache.append(x, x, table, lens)
         assert cache.attention(x, table, lens).shape == x.shape
+
+
+def test_prompts_of_many_heads():
+    """More blocks of query rows times heads than one dimension of a grid holds."""
+    heads, tokens, dim, page = 256, 4200, 16, 64
+    cache = make_cache(70, heads, page, dim, seed=9)
+    table = make_table([tokens + 7], page, 70)
+    q = torch.randn(1, tokens, heads, dim, generator=torch.Generator().manual_seed(9)).cuda().bfloat16()
+    got = cache.attention(q, table, ints([tokens + 7]))
+    n = tokens + 7
+    k, _, _ = values_of(cache, "key", table, 0, n)
+    v, _, step = values_of(cache, "value", table, 0, n)
+    sees = torch.arange(n, device="cuda")[None, :] <= torch.arange(7, n, device="cuda")[:, None]
+    for h in (0, 1, 100, 254, 255):
+        qh = q[0, :, h].double()
+        score = (qh @ k[h].T) * dim**-0.5
+        off = (qh.abs() @ k[h].abs().T * dim**-0.5).masked_fill(~sees, 0).amax(-1, keepdim=True) * (dim / 16 + 8) * 2.0**-23
+        p = torch.softmax(score.masked_fill(~sees, float("-inf")), -1)
+        want = p @ v[h]
+        bound = 2.0**-8 * want.abs() + (p @ v[h].abs()) * (2 * off + 2.0**-11 + 2.0**-17)
+        bound = bound + n * 2.0**-25 * (p * step[h]).amax(-1, keepdim=True) * LEVELS
+        assert bool(((got[0, :, h].double() - want).abs() <= bound).all()), h

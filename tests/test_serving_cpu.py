@@ -139,3 +139,14 @@ def test_cpu_tensors_are_refused():
         Int8KVCache.from_buffers(codes, codes.clone(), torch.zeros(4, 1), torch.zeros(4, 1))
     with pytest.raises(NotImplementedError, match="page_size"):
         Int8KVCache.from_buffers(codes[:, :, :8].contiguous(), codes[:, :, :8].contiguous(), torch.zeros(4, 1), torch.zeros(4, 1))
+
+
+def test_prompts_that_one_grid_does_not_hold_are_taken():
+    """Blocks of sixteen query rows times cache heads: up to 2^20 in one call, with no scratch for so many."""
+    from aimet_b200 import _lib
+
+    for heads, group, tokens in ((8, 4, 32768), (32, 1, 32768), (8, 8, 131072), (1024, 1, 16000)):
+        c = _lib.KVCache(1 << 20, 1 << 20, 1 << 20, 1 << 20, 4096, heads, 64, 128, 0)
+        assert _lib.lib.aimet_b200_kv_attention_scratch_bytes(c, 1, tokens, group, 2048, _lib.AB_BF16) == 0, (heads, group, tokens)
+    c = _lib.KVCache(1 << 20, 1 << 20, 1 << 20, 1 << 20, 4096, 1024, 64, 128, 0)
+    assert _lib.lib.aimet_b200_kv_attention_scratch_bytes(c, 1, 16384, 1, 2048, _lib.AB_BF16) == _lib.AB_ERR_UNSUPPORTED
