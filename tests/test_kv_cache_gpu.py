@@ -661,3 +661,20 @@ def test_prompts_of_many_heads():
         bound = 2.0**-8 * want.abs() + (p @ v[h].abs()) * (2 * off + 2.0**-11 + 2.0**-17)
         bound = bound + n * 2.0**-25 * (p * step[h]).amax(-1, keepdim=True) * LEVELS
         assert bool(((got[0, :, h].double() - want).abs() <= bound).all()), h
+
+
+@pytest.mark.parametrize("vec", [True, False])
+def test_append_special_values_of_float32(vec):
+    """As above for the smaller types: NaN, infinities, blocks of zeros, slices that start off 16 bytes."""
+    cache = make_cache(10, 2, 16, 64)
+    table = make_table([40, 20], 16, 10)
+    at = 0 if vec else 3
+    key = torch.randn(2, 20, 2, 300, device="cuda")[..., at:at + 64]
+    value = torch.randn(2, 2, 20, 64, device="cuda").transpose(1, 2)
+    key[0, 3, 0, 5], key[0, 4, 1, 6], key[1, 2, 0, 0] = float("nan"), float("inf"), float("-inf")
+    value[0, 12:20, 0] = 0
+    value[1, :, 1] = 1e-30
+    value[1, 2, 0, :] = float("inf")
+    check = expected_append(cache, key, value, table, [12, 0], [20, 20])
+    cache.append(key, value, table, ints([12, 0]))
+    check()
