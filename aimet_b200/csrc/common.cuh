@@ -71,6 +71,9 @@ inline int dtype_size(int dt) {
 
 int sm_count();
 
+__host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
 // Programmatic dependent launch: a kernel launched through launch_pdl may become resident while
 // its predecessor in the stream is still draining; it must execute pdl_prologue() before it
 // touches global memory (the wait returns once the predecessor has completed and its writes are

@@ -13,8 +13,6 @@ constexpr int kTileK = 64;    // input channels per tile
 constexpr int kChunkK = 256;  // input channels per chunk: four tiles, 2 KB that one warp requests at once
 constexpr int64_t kMaxK = 1ll << 20;
 
-__host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // Codes [channel tile][tile of columns][lane][16 bytes]; scales (float32, or uint8 factors) and zero points
 // (int8) [channel tile][chunk][entry][channel][sub]: one entry per chunk (blocks of 256 columns or more), two
 // (128) or four (64 or fewer, with 64 / block neighbouring blocks in an entry).  What lies behind the matrix

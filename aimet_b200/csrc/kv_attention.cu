@@ -79,8 +79,6 @@ struct AttnArgs {
     float scale_log2;  // softmax scale * log2(e)
 };
 
-__host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -91,7 +89,6 @@ __device__ __forceinline__ float log2_fast(float x) {
     asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -692,7 +689,7 @@ struct Cut {
     bool cluster;  // the pieces of a row block are a cluster of CTAs; otherwise they leave partial results in scratch
 };
 int padded_dim(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
-Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens, int64_t table_width, int io_dtype) {
+Cut cut_of(int heads, int dim, int group, int page, int64_t seqs, int64_t tokens, int64_t table_width) {
     Cut c;
     const int64_t rows = tokens * group;
     // Sixteen rows per CTA share the converted codes.  (Thirty-two leave registers for two CTAs of four warps on an SM
@@ -784,7 +781,7 @@ extern "C" int64_t aimet_b200_kv_attention_scratch_bytes(const ab_kv_cache *cach
     const int rc = check_call(cache, seqs, tokens, group, table_width, io_dtype);
     if (rc != AB_OK) return rc;
     if (seqs == 0 || tokens == 0) return 0;
-    const Cut c = cut_of(cache->num_heads, cache->head_dim, (int)group, cache->page_size, seqs, tokens, table_width, io_dtype);
+    const Cut c = cut_of(cache->num_heads, cache->head_dim, (int)group, cache->page_size, seqs, tokens, table_width);
     if (c.cluster) return 0;
     return seqs * cache->num_heads * c.row_blocks * c.pieces * 8 * c.eights * (int64_t)(cache->head_dim + 4) * 4;
 }
@@ -804,7 +801,7 @@ extern "C" int aimet_b200_kv_attention(const ab_kv_cache *cache, const void *que
     if (!aligned16(out)) return fail(AB_ERR_INVALID, "out must be 16-byte aligned");
     if (need > 0 && (!scratch || scratch_bytes < need || !aligned16(scratch)))
         return fail(AB_ERR_SCRATCH, "scratch of %lld bytes, 16-byte aligned, is needed (got %lld)", (long long)need, (long long)scratch_bytes);
-    const Cut cut = cut_of(cache->num_heads, cache->head_dim, (int)group, cache->page_size, seqs, tokens, table_width, io_dtype);
+    const Cut cut = cut_of(cache->num_heads, cache->head_dim, (int)group, cache->page_size, seqs, tokens, table_width);
     AttnArgs a;
     a.key = static_cast<const int8_t *>(cache->key);
     a.value = static_cast<const int8_t *>(cache->value);

@@ -23,8 +23,6 @@ struct CacheView {
     int heads, page, dim;
 };
 
-__host__ __device__ inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
-
 // ---------------------------------------------------------------------------------------------------
 // append
 //
