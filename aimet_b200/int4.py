@@ -217,7 +217,7 @@ class PackedInt4Weight:
         with torch.no_grad():
             if scale.dim() > 2:
                 raise NotImplementedError(f"scales of shape {tuple(scale.shape)} for a linear layer's weight")
-            codes = _simulated_codes(weight.detach(), encoding)
+            codes = _simulated_codes(weight, encoding)
             if not bool(torch.isfinite(codes).all()):
                 raise NotImplementedError("a weight or scale that is not a number has no codes")
 

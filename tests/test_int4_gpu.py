@@ -606,3 +606,25 @@ def test_scales_near_the_end_of_the_range(dtype, tokens, grid):
     w = dequantized(codes, scale, offset, int_scale)
     got = linear_int4(x, packed_of(codes, scale, offset, qmin, int_scale))
     assert_close(got, x, w, weight_in_16=tokens > 8 and dtype != torch.float32)
+
+
+def test_packed_codes_are_the_simulated_ones_while_gradients_are_spiked():
+    """With pivot gradient spiking on, a trainable weight is simulated by division in its own type, a frozen one by
+    the fake-quantize arithmetic."""
+    from aimet_b200 import nn as qnn
+    from aimet_b200 import pgs
+
+    model = layers_of(torch.bfloat16, sizes=((256, 384, False),))
+    x = torch.eye(256, device="cuda").bfloat16()
+    pgs.enable_pgs()
+    try:
+        for trainable in (True, False):
+            model[0].layer.weight.requires_grad_(trainable)
+            with torch.no_grad():
+                with qnn.precomputed(model):
+                    want = model(x).double()
+                with qnn.precomputed(model, packed=True):
+                    got = model(x).double()
+            assert bool(((got - want).abs() <= 3 * 2.0**-8 * want.abs()).all()), trainable
+    finally:
+        pgs.disable_pgs()
