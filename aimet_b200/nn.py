@@ -56,7 +56,7 @@ class QuantizedLayer(nn.Module):
         packed = self.__dict__.get("_packed_weight")
         bias = self.layer.bias
         if (packed is not None and not torch.is_grad_enabled() and getattr(qw, "_observer_hook", None) is None
-                and not has_tangent(x, bias)):
+                and not has_tangent(x, bias) and not torch._C._functorch.is_functorch_wrapped_tensor(x)):  # pylint: disable=protected-access
             if torch.is_autocast_enabled("cuda"):  # the types that autocast gives the plain product
                 dtype = torch.get_autocast_dtype("cuda")
                 x = x.to(dtype) if x.is_floating_point() and x.dtype != torch.float64 else x

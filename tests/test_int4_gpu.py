@@ -628,3 +628,17 @@ def test_packed_codes_are_the_simulated_ones_while_gradients_are_spiked():
             assert bool(((got - want).abs() <= 3 * 2.0**-8 * want.abs()).all()), trainable
     finally:
         pgs.disable_pgs()
+
+
+def test_packed_layers_under_vmap():
+    """Tensors that torch.func wraps have no data of their own: the simulated weight is used."""
+    from aimet_b200 import nn as qnn
+
+    model = layers_of(torch.float32)
+    x = torch.randn(5, 3, 64, device="cuda")
+    with torch.no_grad():
+        with qnn.precomputed(model):
+            want = torch.func.vmap(model)(x)
+        with qnn.precomputed(model, packed=True):
+            got = torch.func.vmap(model)(x)
+    assert torch.equal(got, want)
