@@ -15,8 +15,8 @@
 // (movmatrix).  More rows are further columns that share the converted codes.  The scales
 // never touch an element: a tile of 16 tokens lies in one page, so the key scale multiplies the scores,
 // and log2 of the value scale is added to the exponent of the weights that multiply V.
-// Measured: 64 contexts of 1000 to 4000 tokens, 8 heads of 128 for 32 query heads, 87 us of 55 (4.0 TB/s; 135 with query
-// rows as the 16-row operand), 2 of 131072 tokens 98 to 101 us of 71 (4.6 TB/s); issue slots 58 % taken.
+// Measured: 64 contexts of 1000 to 4000 tokens, 8 heads of 128 for 32 query heads, 86 us of 55 (4.1 TB/s; 135 with query
+// rows as the 16-row operand), 2 of 131072 tokens 100 us of 71 (4.6 TB/s); issue slots 57 % taken.
 //
 // Precision: q is scaled by a power of two per row into float16's range (exact for float16 and
 // bfloat16; what a bfloat16 row loses below 2^-39 of its largest element does not reach a float32 sum);
@@ -47,12 +47,13 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStages = 4;
 constexpr int kTokens = 16;     // per tile
-// Tokens of a piece at least: two tiles per warp where contexts are short (one of 500 tokens: 8.2 us with pieces
-// of 128, 9.5 with 256, 9.2 uncut), up to 512 where they are long and joining many pieces would cost more
-// than it gains (8000 tokens: 13.8 us with 512, 15.2 with 192).
+// Tokens of a piece at least: two tiles per warp where contexts are short (one of 500 tokens: 5.9 us with pieces
+// of 128, 7.1 with 256, 8.0 uncut), up to 512 where they are long (one of 32000: 30.1 us with 512 or 192 at most, 32.2
+// with 1024; 8000 in a table for 131072: 19.7, 19.2 and 19.7).
 constexpr int kMinPiece = 128, kMaxMinPiece = 512;
-// Pieces per CTA slot of the machine: one where pieces are all that fills it (two of 131072 tokens: 108 us, 119 with
-// two); three where sequences and heads do, so that ragged lengths even out (64 of 1000 to 4000: 99 us, 106 with one).
+// Pieces per CTA slot of the machine: one where pieces are all that fills it (two of 131072 tokens: 112 us, 118 with
+// two; 8000 in a table for 131072: 19.7 and 25.3); three where sequences and heads do, so that ragged lengths even out
+// (64 of 1000 to 4000: 79 us, 82 with one).
 constexpr int kWaves = 3;
 constexpr int kMostCluster = 8, kClusterPiece = 1024;
 

@@ -88,7 +88,7 @@ def _simulated_codes(weight: torch.Tensor, encoding) -> torch.Tensor:
     """The codes whose values ``quantize_dequantize`` gives for a weight when no gradient is wanted.  That is what
     ``quantize`` gives, except where the fake-quantize arithmetic runs (per tensor and per channel): there the
     weight is multiplied by 1 / scale in float32 whatever its type, while ``quantize`` divides in the weight's
-    type, and quotients near the middle of two codes (in bfloat16 one of a hundred) fall differently."""
+    type, and quotients near the middle of two codes (in bfloat16 one of sixty) fall differently."""
     scale, offset, qmin, qmax, block = encoding.scale, encoding.offset, encoding.qmin, encoding.qmax, encoding.block_size
     if not backend._takes_fake_quantize_path(weight, scale, offset, block, 0.0, qmin, qmax):  # pylint: disable=protected-access
         return backend.quantize(weight, scale, offset, qmin, qmax, block)
@@ -251,7 +251,9 @@ def linear_int4(input: torch.Tensor, weight: PackedInt4Weight, bias: Optional[to
 
     float32, float16 or bfloat16 activations; sums in float32, one rounding to ``input.dtype``.  A few
     tokens, and float32 always, multiply the integer codes exactly; many tokens multiply weights that are
-    rounded to the 16-bit type once, as a simulated 16-bit model's are.  Rows of up to 37120 input features in
+    rounded to the 16-bit type once, as a simulated 16-bit model's are.  Which of the two runs depends on the
+    number of tokens and input features (from 17 tokens on the second; with long rows from three on, where
+    they start on 16 bytes).  Rows of up to 37120 input features in
     float32 and 111360 in 16 bits.  For inference: an input or bias that needs a gradient, or carries a
     forward-mode derivative, is refused (train through the quantizer instead).
     """

@@ -35,7 +35,8 @@ class Int8KVCache:
     """``num_pages`` pages of ``page_size`` tokens for ``num_heads`` key / value heads of ``head_dim``.
 
     ``key``, ``value``: int8 ``[num_pages, num_heads, page_size, head_dim]``, codes in [-127, 127];
-    ``key_scale``, ``value_scale``: float32 ``[num_pages, num_heads]``; a code stands for ``code * scale``.
+    ``key_scale``, ``value_scale``: float32 ``[num_pages, num_heads]``, not negative; a code stands for
+    ``code * scale``.
     ``page_size`` is a multiple of 16 up to 1024, ``head_dim`` a multiple of 16 up to 256.
     """
 
@@ -51,7 +52,7 @@ class Int8KVCache:
     @classmethod
     def from_buffers(cls, key: torch.Tensor, value: torch.Tensor, key_scale: torch.Tensor,
                      value_scale: torch.Tensor) -> "Int8KVCache":
-        """A cache over existing buffers (used in place; shapes and dtypes as in the class)."""
+        """A cache over four existing buffers that share no memory (used in place; shapes and dtypes as in the class)."""
         if key.dim() != 4:
             raise RuntimeError(f"key must be [num_pages, num_heads, page_size, head_dim], got shape {tuple(key.shape)}")
         for name, t, dtype, shape in (("key", key, torch.int8, key.shape), ("value", value, torch.int8, key.shape),
@@ -154,7 +155,8 @@ class Int8KVCache:
         the new grid: a token ends within 2.5 steps of its value, within half a step if its block was
         written at once.  NaN is stored as zero; infinities as the block's largest level, scales being taken
         from finite values.  Tokens whose table entry is outside ``[0, num_pages)``, or lies behind the
-        table's end, are dropped.  Within a call no page may receive tokens of two sequences.
+        table's end, are dropped.  Within a call no page may receive tokens of two sequences, or of two blocks
+        of one.
         """
         if _calls is not None and _calls.append(key, value, block_table, context_lens, new_lens, self._address, self._index):
             return
@@ -249,7 +251,9 @@ class Int8KVCache:
         (default: all).  Query ``i`` stands at position ``context_lens - query_lens + i`` and sees positions
         up to its own (``causal``) and after its own minus ``window``, as far as they have a page (positions behind
         the table's end have none); ``scale`` defaults to
-        ``head_dim ** -0.5``.  Scores, softmax and sums are float32.
+        ``head_dim ** -0.5``.  Scores, softmax and sums are float32; float32 queries keep 22 bits.  A token's weight
+        is rounded to 11 bits before it multiplies its value (float32 queries: 22), and by at most 2^-40 of the
+        largest product of a weight and its value's scale.
 
         Returns ``[sequences, tokens, heads, head_dim]`` in ``query.dtype``; queries that see nothing, and
         those behind ``query_lens``, give zeros.  With ``return_lse`` also the logarithm of each query's

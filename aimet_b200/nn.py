@@ -215,7 +215,9 @@ def precomputed(model: nn.Module, packed: bool = False):
     (:class:`aimet_b200.int4.PackedInt4Weight`) instead of the quantize-dequantized weight, a quarter of
     its bytes in 16 bits, and multiply with them directly in no-grad forwards, in the types that autocast
     asks for where it is on.  Grids that cannot be packed, and layers of other kinds, are held as without
-    ``packed``."""
+    ``packed``.  Packed layers are for decoding: on a B200 a 14336 x 4096 layer takes 10 us instead of 22
+    for one token in bfloat16, 18 instead of 21 for 16, 31 instead of 24 for 128 and 153 instead of 130 for 1500;
+    in float32 18 instead of 75 for one, 196 instead of 167 for 64 and 4270 instead of 3010 for 1500."""
     from .quantizer import derive_encodings
 
     with contextlib.ExitStack() as stack, torch.no_grad():

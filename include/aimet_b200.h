@@ -431,7 +431,7 @@ int aimet_b200_int4_linear(const ab_int4_weight *weight, const void *x, int64_t 
  * reference.  value of a code = code * scale, one scale per page (a block of page_size tokens)
  * and head:
  *   key, value              int8 [num_pages][num_heads][page_size][head_dim], 16-byte aligned
- *   key_scale, value_scale  float32 [num_pages][num_heads]
+ *   key_scale, value_scale  float32 [num_pages][num_heads], not negative
  * Token j of sequence s lives in row j % page_size of page block_table[s][j / page_size]
  * (int32, rows table_stride apart, table_width entries).  Entries outside [0, num_pages) mean "no
  * page": nothing is written there, reads give zeros, attention masks the tokens.  page_size is a
@@ -449,7 +449,7 @@ typedef struct ab_kv_cache {
  * a new token gets scale = max|x| * float32(1 / 127) over its new tokens' finite values; a partly filled
  * one keeps its scale if that is at least as large and else gets max(max|x| * float32(1 / 127), 1.25 * scale), the codes in
  * it becoming rint(code * (old / new)).  code = clamp(rint(x / scale), -127, 127); NaN is stored as
- * zero.  Two sequences of a call must not append into the same page. */
+ * zero.  Two sequences of a call, or two blocks of one, must not append into the same page. */
 int aimet_b200_kv_append(const ab_kv_cache *cache, const void *key, const void *value, const int64_t *key_strides,
                          const int64_t *value_strides, int64_t seqs, int64_t tokens, const int32_t *block_table,
                          int64_t table_stride, int64_t table_width, const int32_t *context_lens,
